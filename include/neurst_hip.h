@@ -576,6 +576,95 @@ typedef struct {
 } NstPack2dJob;
 int nst_pack2d(const NstPack2dJob* jobs_dev, int njobs, int total_blocks, void* stream);
 
+/* ------------------------------------------------------------------ paged key / value caches of incremental decoding
+ * The reference grows a dense [B, t, d] key / value tensor per layer by concatenation and gathers all of it behind every beam-search
+ * step (neurst/layers/attentions/multi_head_attention.py:254-290, neurst/layers/search/beam_search.py:409-410).  Here a cache may be
+ * PAGED: k_pool / v_pool hold num_pages pages of page_size token rows, block_table[b][j] (int32, [B, max_pages], row stride
+ * table_stride) is the page that holds tokens j * page_size .. of request b, and the SLOT of a token is
+ * page * page_size + position % page_size.  Requests may have different lengths.
+ * Device-resident indexes (table entries, slots, free pages, parents, spare pages) are range-checked by the kernels: an index outside
+ * its range contributes nothing and is never dereferenced.  All entry points are asynchronous, allocate nothing and may be
+ * captured.  (Additions to ABI 10: nothing that was there changed.) */
+typedef struct {
+  int num_pages, page_size;       /* page_size: any positive number */
+  int dtype;                      /* NST_F32 or NST_BF16: pools, q, k, v and out */
+  int reserved;
+  /* strides in ELEMENTS between pages, the token rows of a page and the heads of a row; a head's dh elements are contiguous.
+   * ([pages, page_size, heads, dh] and [pages, heads, page_size, dh] are both just strides.) */
+  int64_t k_page_stride, k_token_stride, k_head_stride;
+  int64_t v_page_stride, v_token_stride, v_head_stride;
+} NstPagedPool;
+
+/* Pages and slots for the new tokens of every request, from lengths that live on the device (one launch).
+ *   cached_lens [B]: tokens of request b that are cached; new_lens [B]: tokens it gets now (negative counts as 0).
+ *   Request b holds ceil(cached / page_size) pages; the ones it lacks for its new tokens are taken from free_pages [n_free], request
+ *   after request, starting at entry *cursor_in, and entered into its row of block_table (other entries stay as they were).
+ *   slots [max_tokens] int64: the slot of every new token, packed request after request in the order of positions; -1 behind
+ *   the last one.  cu_new [B + 1]: where the tokens of a request start in that order.  seq_lens [B] = cached + new.
+ *   *cursor_out: the first entry of free_pages that is still free.
+ * When the free pages run out or a table row is full, the tokens that have no page get slot -1 and are not counted in seq_lens.
+ * max_tokens should be at least sum(new_lens): tokens behind it get a page but no slot.  The outputs may not be the inputs. */
+int nst_paged_plan(const int32_t* cached_lens, const int32_t* new_lens, int B, int32_t* block_table, int64_t table_stride, int max_pages,
+                   const int32_t* free_pages, int n_free, const int32_t* cursor_in, int page_size, int64_t* slots, int64_t max_tokens,
+                   int32_t* seq_lens, int32_t* cu_new, int32_t* cursor_out, void* stream);
+
+/* Rows k, v [tokens, kv_heads, dh] (strides in elements, e.g. column blocks of a packed projection) into the slots of the pools.
+ * A slot outside [0, num_pages * page_size) is skipped.  No slot may appear twice (which row it would hold is undefined). */
+int nst_paged_append(const void* k, const void* v, int64_t tokens, int kv_heads, int dh, int64_t k_token_stride, int64_t k_head_stride,
+                     int64_t v_token_stride, int64_t v_head_stride, void* k_pool, void* v_pool, const NstPagedPool* pool,
+                     const int64_t* slots, void* stream);
+
+/* Attention of ONE new token per request over its cached tokens (multi_head_attention.py:124-164 with Tq = 1):
+ *   out[b, h] = sum_{t < seq_lens[b]} softmax_t(scale * q[b, h] . k_t[h']) v_t[h'],   h' = h / (H / Hkv)
+ * lse (nullable) [B, H] f32 = log-sum-exp of the scaled scores.  A request with no (valid) token gets out = 0, lse = -inf.  Lengths are
+ * clamped to [0, max_pages * page_size]; tokens behind a request's length are not read.  Scores, softmax statistics and the sums
+ * are f32; with NST_BF16 the probabilities are rounded to bf16 for the product with v.
+ * max_len: a bound of seq_lens that the host knows (0: max_pages * page_size).  It only chooses how the work is split; a longer
+ * request is still attended over in full. */
+typedef struct {
+  int B, H, Hkv, dh;              /* H a multiple of Hkv; 1 <= dh <= 256 */
+  int max_pages, max_len;
+  float scale;
+  int reserved;
+  int64_t q_row_stride, q_head_stride, o_row_stride, o_head_stride;   /* elements */
+  int64_t table_stride;
+  NstPagedPool pool;
+} NstPagedAttnDesc;
+/* bytes of device scratch (16-byte aligned) the call needs; 0: none, negative: NST_ERR_* */
+int64_t nst_paged_attention_workspace_bytes(const NstPagedAttnDesc* desc);
+int nst_paged_attention(const NstPagedAttnDesc* desc, const void* q, const void* k_pool, const void* v_pool, const int32_t* block_table,
+                        const int32_t* seq_lens, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Re-ordering behind a beam-search step (tf.gather(cache, beam_ids), beam_search.py:409-410): row r continues the sequence of row
+ * parents[r] (int64), which must be as long as its own.  Full pages are SHARED: only the table row is gathered.  The partly filled
+ * last page of a row whose parent is another row is copied (its seq_len % page_size token rows, in every one of the `planes`
+ * key / value planes) into the row's spare page, which takes its place in the table; the page that row filled before becomes
+ * its new spare.  So every row always writes into a partly filled page of its own, and a re-ordering moves less than a page per row.
+ *   pool: planes x num_pages pages; a page is page_size dense token rows of token_bytes; plane_stride / page_stride in bytes.
+ *   table_out is written in full (-1 behind the last page); spare_out[r] = the spare page of row r afterwards.
+ * Preconditions: spare pages and partly filled pages belong to one row only.  A row whose parent (or spare page, where it needs one)
+ * is out of range or whose parent has another length keeps its own sequence.  The outputs may not overlap the inputs. */
+int nst_paged_reorder(void* pool, int planes, int64_t plane_stride, int num_pages, int64_t page_stride, int page_size, int64_t token_bytes,
+                      const int32_t* table_in, int64_t in_stride, int32_t* table_out, int64_t out_stride, int max_pages, int rows,
+                      const int32_t* seq_lens, const int64_t* parents, const int32_t* spare_in, int32_t* spare_out, void* stream);
+
+/* ------------------------------------------------------------------ log probabilities of given tokens
+ * logits [rows, V] (row stride ldl elements), V <= 2^20.  One read of the logits gives, per row (f32, each output nullable):
+ *   logp = log softmax(logits)[token]   (0 where the token is outside [0, V): padding),   lse = log-sum-exp,
+ *   entropy = -sum p log p,   top_logp / top_ids [rows, top_n]: the top_n <= min(64, V) likeliest tokens in descending order
+ * (tf.nn.log_softmax + tf.nn.top_k of beam_search.py:104-215).  Equal logits rank by the lower id, a NaN ranks first.  A ruled-out
+ * logit (-1e9, -inf) has probability 0 and adds nothing to the entropy; a row of nothing but -inf gives NaN as softmax does.
+ * workspace: nst_token_logprobs_workspace_bytes(...) bytes, 16-byte aligned (0: none needed). */
+int64_t nst_token_logprobs_workspace_bytes(int64_t rows, int V, int top_n, int dtype);
+int nst_token_logprobs_fwd(const void* logits, const int64_t* tokens, float* logp, float* entropy, float* lse, float* top_logp,
+                           int64_t* top_ids, int64_t rows, int V, int64_t ldl, int top_n, int dtype, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+/* dlogits = dlogp * ([j = token] - p_j) - dentropy * p_j * (log p_j + entropy); dlogp, dentropy [rows] f32, each nullable; lse and entropy
+ * as the forward call left them.  dlogits may be logits itself (ldd == ldl), and must not overlap it otherwise.  The alternatives
+ * carry no gradient. */
+int nst_token_logprobs_bwd(const void* logits, const int64_t* tokens, const float* lse, const float* entropy, const float* dlogp,
+                           const float* dentropy, void* dlogits, int64_t rows, int V, int64_t ldl, int64_t ldd, int dtype, void* stream);
+
 /* ---------------------------------------------------------------------------------------------------------------------
  * Gradient exchange over RCCL (one process per GPU; ABI v8).  Replaces the Horovod calls of the reference's data-parallel
  * step: the averaged all-reduce of every gradient (neurst/training/hvd_utils.py:46-62, hvd.DistributedOptimizer /

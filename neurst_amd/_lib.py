@@ -96,6 +96,19 @@ class NstTransposeJob(C.Structure):
                 ("tile0", C.c_int)]
 
 
+class NstPagedPool(C.Structure):
+    _fields_ = [("num_pages", C.c_int), ("page_size", C.c_int), ("dtype", C.c_int), ("reserved", C.c_int),
+                ("k_page_stride", C.c_int64), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+                ("v_page_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64)]
+
+
+class NstPagedAttnDesc(C.Structure):
+    _fields_ = [("B", C.c_int), ("H", C.c_int), ("Hkv", C.c_int), ("dh", C.c_int), ("max_pages", C.c_int), ("max_len", C.c_int),
+                ("scale", C.c_float), ("reserved", C.c_int),
+                ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64), ("o_row_stride", C.c_int64), ("o_head_stride", C.c_int64),
+                ("table_stride", C.c_int64), ("pool", NstPagedPool)]
+
+
 _P, _I, _L, _F, _U64 = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_uint64
 
 # name -> argtypes; every symbol declared in include/neurst_hip.h
@@ -159,6 +172,14 @@ SIGNATURES = {
                               _L, _P, _P, _L, _P],
     "nst_transpose_bf16": [_P, _I, _I, _P],
     "nst_pack2d": [_P, _I, _I, _P],
+    "nst_paged_plan": [_P, _P, _I, _P, _L, _I, _P, _I, _P, _I, _P, _L, _P, _P, _P, _P],
+    "nst_paged_append": [_P, _P, _L, _I, _I, _L, _L, _L, _L, _P, _P, C.POINTER(NstPagedPool), _P, _P],
+    "nst_paged_attention_workspace_bytes": [C.POINTER(NstPagedAttnDesc)],
+    "nst_paged_attention": [C.POINTER(NstPagedAttnDesc), _P, _P, _P, _P, _P, _P, _P, _P, _L, _P],
+    "nst_paged_reorder": [_P, _I, _L, _I, _L, _I, _L, _P, _L, _P, _L, _I, _I, _P, _P, _P, _P, _P],
+    "nst_token_logprobs_workspace_bytes": [_L, _I, _I, _I],
+    "nst_token_logprobs_fwd": [_P, _P, _P, _P, _P, _P, _P, _L, _I, _L, _I, _I, _P, _L, _P],
+    "nst_token_logprobs_bwd": [_P, _P, _P, _P, _P, _P, _P, _L, _I, _L, _L, _I, _P],
     "nst_stream_create": [_I, C.POINTER(C.c_void_p)],
     "nst_stream_destroy": [_P],
     "nst_comm_unique_id": [_P, C.c_size_t],
@@ -181,7 +202,8 @@ def _load():
         fn = getattr(lib, name)  # AttributeError if the symbol is missing -> loud failure
         fn.argtypes = argtypes
         fn.restype = (C.c_char_p if name == "nst_last_error_string"
-                      else C.c_int64 if name in ("nst_attention_dropout_mask_bytes", "nst_ffn_gate_bits_bytes", "nst_ffn_ln_slab_bytes")
+                      else C.c_int64 if name in ("nst_attention_dropout_mask_bytes", "nst_ffn_gate_bits_bytes", "nst_ffn_ln_slab_bytes",
+                                           "nst_paged_attention_workspace_bytes", "nst_token_logprobs_workspace_bytes")
                       else C.c_uint32 if name == "nst_crc32c" else C.c_int)
     ver = lib.nst_abi_version()
     if ver != NST_ABI_VERSION:

@@ -583,7 +583,8 @@ _NAMES = ["layernorm_fwd", "layernorm_bwd", "add_layernorm_fwd", "add_layernorm_
           "cast_f32_to_bf16", "ffn_supported", "ffn_fwd", "ffn_bwd", "transpose_bf16", "pack2d",
           "dropout_seed_offset_bind", "dropout_seed_offset_set", "dropout_seed_offset_add", "loss_scale_update", "splitk_reduce_multi",
           "gemm_wgrad_group", "seq_mask", "xent_reduce", "rowgemm_supported", "gemm_add_layernorm_fwd", "gemm_layernorm_bwd",
-          "gemm_rowdot256", "ffn_ln_supported", "ffn_add_layernorm_fwd", "ffn_layernorm_bwd"]
+          "gemm_rowdot256", "ffn_ln_supported", "ffn_add_layernorm_fwd", "ffn_layernorm_bwd",
+          "paged_plan", "paged_append", "paged_attention", "paged_reorder", "token_logprobs", "token_logprobs_bwd"]
 
 
 def seq_mask(lengths, max_len, on_token, on_padding, halvings=0, stride=2):
@@ -598,6 +599,106 @@ def xent_reduce(xent, weights):
     B, L = weights.shape
     nll, tok = xent.reshape(B, L).to(F64).sum(1), weights.to(F64).sum(1)
     return nll.float(), tok.float(), (nll.sum() / tok.sum()).float().reshape(1), (1.0 / tok.sum()).float().reshape(1)
+
+
+# ---------------------------------------------------------------------------------------------------- paged caches
+def paged_plan(cached_lens, new_lens, block_table, free_pages, cursor, page_size, max_tokens):
+    W, cap = block_table.shape[1], block_table.shape[1] * page_size
+    at, n_free = max(int(cursor), 0), free_pages.shape[0]
+    slots, seq, cu, t = torch.full((int(max_tokens),), -1, dtype=torch.int64), [], [0], 0
+    for b in range(cached_lens.shape[0]):
+        cached, new = min(max(int(cached_lens[b]), 0), cap), max(int(new_lens[b]), 0)
+        held = -(-cached // page_size)
+        need = -(-min(cached + new, cap) // page_size) - held
+        got = min(max(n_free - at, 0), need)
+        block_table[b, held:held + got] = free_pages[at:at + got]
+        at += need
+        seq.append(min(cached + new, (held + got) * page_size))
+        for pos in range(cached, cached + new):
+            if t < max_tokens and pos // page_size < held + got:
+                page = int(block_table[b, pos // page_size])
+                slots[t] = page * page_size + pos % page_size if page >= 0 else -1
+            t += 1
+        cu.append(t)
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32)      # noqa: E731
+    return slots, i32(seq), i32(cu), i32([min(at, max(n_free, int(cursor)))])
+
+
+def paged_append(k, v, k_pool, v_pool, slots):
+    ps = k_pool.shape[1]
+    for t, s in enumerate(slots.tolist()):
+        if 0 <= s < k_pool.shape[0] * ps:
+            k_pool[s // ps, s % ps], v_pool[s // ps, s % ps] = k[t], v[t]
+
+
+def paged_attention(q, k_pool, v_pool, block_table, seq_lens, scale=None, max_len=None, return_lse=False):
+    B, H, dh = q.shape
+    P, ps, Hk = k_pool.shape[:3]
+    scale = dh ** -0.5 if scale is None else scale
+    out, lse = torch.zeros(B, H, dh, dtype=F64), torch.full((B, H), -float("inf"), dtype=F64)
+    for b in range(B):
+        n = min(max(int(seq_lens[b]), 0), block_table.shape[1] * ps)
+        pos = [(int(block_table[b, t // ps]), t % ps) for t in range(n)]
+        pos = [(p, o) for p, o in pos if 0 <= p < P]
+        if not pos:
+            continue
+        pi, oi = torch.tensor([p for p, _ in pos]), torch.tensor([o for _, o in pos])
+        k, v = k_pool[pi, oi].to(F64), v_pool[pi, oi].to(F64)                       # [n, Hk, dh]
+        for h in range(H):
+            s = (k[:, h // (H // Hk)] @ q[b, h].to(F64)) * scale
+            lse[b, h] = torch.logsumexp(s, 0)
+            out[b, h] = torch.softmax(s, 0) @ v[:, h // (H // Hk)]
+    return (out.to(q.dtype), lse.float()) if return_lse else out.to(q.dtype)
+
+
+def paged_reorder(pool, block_table, seq_lens, parents, spare):
+    N, P, ps = pool.shape[:3]
+    R, W = block_table.shape
+    before, table, left = pool.clone(), torch.full_like(block_table, -1), spare.clone()
+    lens = [min(max(int(n), 0), W * ps) for n in seq_lens]
+    for r in range(R):
+        p, n = int(parents[r]), lens[r]
+        if not 0 <= p < R or lens[p] != n:
+            p = r
+        last = n // ps
+        move = p != r and n % ps > 0
+        if move and not (0 <= int(block_table[p, last]) < P and 0 <= int(spare[r]) < P):
+            p, move = r, False
+        used = -(-n // ps)
+        table[r, :used] = block_table[p, :used]
+        if move:
+            pool[:, int(spare[r]), :n % ps] = before[:, int(block_table[p, last]), :n % ps]
+            table[r, last], left[r] = spare[r], block_table[r, last]
+    return table, left
+
+
+# ---------------------------------------------------------------------------------------------------- token log probabilities
+def token_logprobs(logits, tokens, top_n=0):
+    x = logits.to(F64)
+    lse = torch.logsumexp(x, -1)
+    lp = x - lse[:, None]
+    p = lp.exp()
+    entropy = -torch.where(p > 0, p * lp, torch.where(p == 0, torch.zeros_like(p), p)).sum(-1)
+    given = (tokens >= 0) & (tokens < x.shape[1])
+    logp = torch.where(given, lp.gather(1, tokens.clamp(0, x.shape[1] - 1)[:, None])[:, 0], torch.zeros_like(lse))
+    ids = torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :top_n].contiguous()
+    return logp.float(), entropy.float(), lse.float(), lp.gather(1, ids).float(), ids
+
+
+def token_logprobs_bwd(logits, tokens, lse, entropy, dlogp, dentropy=None, out=None):
+    x = logits.to(F64)
+    lp = x - lse.to(F64)[:, None]
+    p = lp.exp()
+    given = (tokens >= 0) & (tokens < x.shape[1])
+    a = torch.zeros_like(lse, dtype=F64) if dlogp is None else torch.where(given, dlogp.to(F64), torch.zeros_like(lse, dtype=F64))
+    g = -p * a[:, None]
+    if dentropy is not None:
+        g = g - torch.where(p == 0, torch.zeros_like(p), p * (lp + entropy.to(F64)[:, None])) * dentropy.to(F64)[:, None]
+    rows = torch.arange(x.shape[0])[given]
+    g[rows, tokens[given]] += a[given]
+    if out is None:
+        return g.to(logits.dtype)
+    return out.copy_(g.to(logits.dtype))
 
 
 def gemm_wgrad_group(items, table=None):
