@@ -583,7 +583,7 @@ int nst_pack2d(const NstPack2dJob* jobs_dev, int njobs, int total_blocks, void* 
  * table_stride) is the page that holds tokens j * page_size .. of request b, and the SLOT of a token is
  * page * page_size + position % page_size.  Requests may have different lengths.
  * Device-resident indexes (table entries, slots, free pages, parents, spare pages) are range-checked by the kernels: an index outside
- * its range contributes nothing and is never dereferenced.  All entry points are asynchronous, allocate nothing and may be
+ * its range contributes nothing and is never dereferenced.  max_pages * page_size <= 2^30.  All entry points are asynchronous, allocate nothing and may be
  * captured.  (Additions to ABI 10: nothing that was there changed.) */
 typedef struct {
   int num_pages, page_size;       /* page_size: any positive number */

@@ -4,12 +4,15 @@
 // A cache holds `num_pages` pages of `page_size` token rows; page p of request b's sequence is block_table[b][p].  The slot of a
 // token is page * page_size + position % page_size.  Every entry read from a table, a slot map, a free list or a list of parents
 // is checked against its range on the device before it becomes an address: an entry outside contributes nothing.
+#include <type_traits>
+
 #include "nst_common.h"
 
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
+constexpr int64_t MAX_POSITIONS = 1 << 30;     // of one request: position arithmetic, a tile or two past the end included, stays in 32 bits
 
 // ---------------------------------------------------------------------------------------------
 // plan
@@ -166,62 +169,349 @@ __global__ void __launch_bounds__(256) paged_append_kernel(AppendParams p) {
 // ---------------------------------------------------------------------------------------------
 // attention of one new token
 // ---------------------------------------------------------------------------------------------
+// A workgroup owns one part of one request's tokens for one key / value head and up to 16 of the query heads that share it; its four
+// waves take tiles of 16 * NF tokens in turn, each with a running maximum and sum of its own, and are joined in LDS at the end.
+// Parts of a request are joined by a second small kernel.
+//   scores   S^T[token][head] = K . Q^T   the 16 x 16 accumulator block of a wave keeps, in lane l, head l & 15 and tokens 4 (l >> 4) + 0..3:
+//   output   O^T[dim][head] += V^T . P^T  ... which is the operand layout of the second product, so the weights stay in registers.
+// K goes from memory straight into operand registers (lane: token l & 15, 16 bytes of its row).  bf16: V rows go through LDS, because
+// their operand needs 8 tokens of one dim per lane (ds_read_b64_tr_b16); f32: the 16x16x4 product takes ONE token per lane, so 16-byte
+// pieces of V rows are operands as they come and nothing passes through LDS.  The waves never wait for each other inside the loop.
+constexpr int MIN_PART = 128;      // tokens: one tile for each wave
+
+__host__ __device__ __forceinline__ int part_tokens(int len, int nsplit) {
+  const int even = (int)(((int64_t)len + nsplit - 1) / nsplit), p = (even + MIN_PART - 1) / MIN_PART * MIN_PART;
+  return p < MIN_PART ? MIN_PART : p;
+}
+
 struct PagedAttnParams {
-  const void *q, *k, *v;
-  void* out;
+  const char *q, *k, *v;
+  char* out;
   float* lse;
   const int32_t *table, *lens;
   int B, H, Hkv, dh, page_size, num_pages, max_pages;
-  int64_t q_row, q_head, o_row, o_head, table_stride;
-  int64_t k_page, k_tok, k_head, v_page, v_tok, v_head;
-  float scale;
+  int64_t q_row, q_head, o_row, o_head, table_stride;               // elements
+  uint32_t k_page, k_tok, v_page, v_tok;                            // elements, below 2^31
+  int64_t k_head, v_head;
+  float scale_log2;
+  int nsplit, qchunks;
+  uint32_t div_magic;      // t / page_size = (t * magic) >> (32 + shift) for 0 <= t < 2^31; 0: pages of one token
+  int div_shift;
+  float* part;             // [B * H][nsplit][dh + 2]: output, maximum, sum of a part
 };
 
-// One wave per (request, head): a lane scores one key of a 64-key step, the lanes then share the head's columns.
 template <typename T>
-__global__ void __launch_bounds__(64) paged_attn_kernel(PagedAttnParams p) {
-  __shared__ float s_p[64];
-  __shared__ int64_t s_v[64];
-  const int lane = threadIdx.x, h = blockIdx.x % p.H, b = blockIdx.x / p.H, hk = h / (p.H / p.Hkv);
-  const T* q = (const T*)p.q + b * p.q_row + h * p.q_head;
-  const int len = min(max(p.lens[b], 0), p.max_pages * p.page_size);
-  float m = -3.402823466e38f, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int t0 = 0; t0 < len; t0 += 64) {
-    const int t = t0 + lane;
-    int page = -1;
-    if (t < len) page = p.table[b * p.table_stride + t / p.page_size];
-    const bool ok = page >= 0 && page < p.num_pages;
-    float s = -INFINITY;
-    if (ok) {
-      const T* k = (const T*)p.k + page * p.k_page + (t % p.page_size) * p.k_tok + hk * p.k_head;
-      s = 0.f;
-      for (int d = 0; d < p.dh; ++d) s += to_f32<T>(q[d]) * to_f32<T>(k[d]);
-      s *= p.scale * LOG2E;
-    }
-    const float mn = fmaxf(m, wave_max(s)), pr = ok ? exp2f(s - mn) : 0.f, back = exp2f(m - mn);
-    l = l * back + pr;
-    m = mn;
-    s_p[lane] = pr;
-    s_v[lane] = ok ? page * p.v_page + (t % p.page_size) * p.v_tok + hk * p.v_head : -1;
-    __syncthreads();
+struct PA;
+template <>
+struct PA<bf16_t> { static constexpr int E = 8; };
+template <>
+struct PA<float> { static constexpr int E = 4; };
+
+// 16 bytes of a row from element d on.  A piece behind the row's end (d >= dh) repeats its first one: the loads have no masks, so that
+// the compiler can keep count of what is in flight; what they may not contribute is zeroed where it is used.
+template <typename T, bool VEC>
+__device__ __forceinline__ uint4 row_chunk(const T* row, int d, int dh) {
+  if (VEC) return *reinterpret_cast<const uint4*>(row + (d < dh ? d : 0));
+  T e[PA<T>::E];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int d = c * 64 + lane;
-      if (d < p.dh) {
-        float a = acc[c] * back;
-        for (int i = 0; i < min(64, len - t0); ++i)
-          if (s_v[i] >= 0) a += s_p[i] * to_f32<T>(((const T*)p.v)[s_v[i] + d]);
-        acc[c] = a;
+  for (int i = 0; i < PA<T>::E; ++i) {
+    const T v = row[d + i < dh ? d + i : 0];
+    e[i] = d + i < dh ? v : T(0);
+  }
+  uint4 r;
+  memcpy(&r, e, 16);
+  return r;
+}
+__device__ __forceinline__ uint4 keep_if(uint4 v, bool ok) { return make_uint4(ok ? v.x : 0u, ok ? v.y : 0u, ok ? v.z : 0u, ok ? v.w : 0u); }
+
+// DP: head size padded to the tile (32, 64, 128, 256); NF: 16-token blocks of a tile
+// VEC: rows are whole 16-byte pieces; EXACT: dh == DP
+template <typename T, int DP, int NF, bool VEC, bool EXACT>
+__global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnParams p) {
+  const int dh = EXACT ? DP : p.dh;
+  constexpr bool BF = sizeof(T) == 2;
+  constexpr int TK = 16 * NF;                          // tokens of a tile
+  constexpr int RSV = DP * 2 + 32;                     // LDS row of V (bf16): rows spread over the banks for the transpose read
+  constexpr int KC = DP * (int)sizeof(T) / 64;         // 16-byte pieces of a K row per lane
+  constexpr int VC = BF ? TK * DP / 8 / 64 : 0;        // 16-byte pieces of the V tile per lane
+  constexpr int NA = DP / 16;                          // accumulator blocks
+  constexpr int WAVE_BYTES = BF ? TK * RSV : 0, JOIN_BYTES = 4 * 16 * (DP + 4) * 4;
+  constexpr int LDS_BYTES = 4 * WAVE_BYTES > JOIN_BYTES ? 4 * WAVE_BYTES : JOIN_BYTES;
+  __shared__ __attribute__((aligned(16))) char lds[LDS_BYTES];
+  __shared__ float s_ml[2][4][16];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, lc = lane & 15;
+  const int heads = p.Hkv * p.qchunks;
+  const int hq = blockIdx.x % heads, rest = blockIdx.x / heads, split = rest % p.nsplit, b = rest / p.nsplit;
+  const int hk = hq / p.qchunks, qc = hq % p.qchunks, group = p.H / p.Hkv;
+  const int h0 = hk * group + qc * 16, nh = min(16, group - qc * 16);
+  const int cap = p.max_pages * p.page_size;
+  const int len = min(max(p.lens[b], 0), cap);
+  const int part = part_tokens(len, p.nsplit), t_begin = split * part, t_end = min(len, t_begin + part);
+  if (t_begin >= len && (p.nsplit > 1 || len > 0)) return;      // (an empty request with one part writes its zeros below)
+  const int32_t* table = p.table + (int64_t)b * p.table_stride;
+  const T* kbase = (const T*)p.k + hk * p.k_head;
+  const T* vbase = (const T*)p.v + hk * p.v_head;
+
+  uint4 qf[KC];
+  {
+    const T* q = (const T*)p.q + (int64_t)b * p.q_row + (int64_t)(h0 + min(lc, nh - 1)) * p.q_head;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const int d = c * (64 / (int)sizeof(T)) + g * PA<T>::E;
+      qf[c] = keep_if(row_chunk<T, VEC>(q, d, dh), lc < nh && d < dh);
+    }
+  }
+  floatx4_t acc[NA];
+#pragma unroll
+  for (int i = 0; i < NA; ++i) acc[i] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+  float m = -3.402823466e38f, l = 0.f;
+  uint4 kr[NF][KC], vr[BF ? VC : NF * 4 * (DP / 64 > 0 ? DP / 64 : 1)];
+
+  // Lane i looks up the page of token t0 + i % TK.  The entry is checked where it is used, a tile later: a check here would wait for it,
+  // and with it for all rows requested before.
+  const int tl = lane % TK;
+  auto look = [&](int t0, int& entry, int& off) __attribute__((always_inline)) {
+    const int t = min(t0 + tl, t_end - 1);
+    const int j = p.div_magic ? (int)(__umulhi((uint32_t)t, p.div_magic) >> p.div_shift) : t;
+    off = t - j * p.page_size;
+    entry = table[j];
+  };
+  // page of this lane's token, 0 (whose rows exist) with the token out of `valid` when it has none
+  auto resolve = [&](int t0, int entry, uint64_t& valid) __attribute__((always_inline)) {
+    const bool ok = t0 + tl < t_end && entry >= 0 && entry < p.num_pages;
+    valid = __ballot(ok);
+    return ok ? entry : 0;
+  };
+  auto load = [&](int page, int off) __attribute__((always_inline)) {
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      const uint32_t pg = __shfl(page, f * 16 + lc, 64), of = __shfl(off, f * 16 + lc, 64);
+      const T* row = kbase + ((uint64_t)pg * p.k_page + (uint64_t)of * p.k_tok);
+#pragma unroll
+      for (int c = 0; c < KC; ++c) kr[f][c] = row_chunk<T, VEC>(row, c * (64 / (int)sizeof(T)) + g * PA<T>::E, dh);
+    }
+    if constexpr (BF) {
+#pragma unroll
+      for (int i = 0; i < VC; ++i) {
+        const int r = (i * 64 + lane) / (DP / 8), col = (i * 64 + lane) % (DP / 8);
+        const uint32_t pg = __shfl(page, r, 64), of = __shfl(off, r, 64);
+        vr[i] = row_chunk<T, VEC>(vbase + ((uint64_t)pg * p.v_page + (uint64_t)of * p.v_tok), col * 8, dh);
+      }
+    } else {
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = f * 16 + g * 4 + r;
+          const uint32_t pg = __shfl(page, key, 64), of = __shfl(off, key, 64);
+          const T* row = vbase + ((uint64_t)pg * p.v_page + (uint64_t)of * p.v_tok);
+#pragma unroll
+          for (int c = 0; c < DP / 64; ++c) vr[(f * 4 + r) * (DP / 64) + c] = row_chunk<T, VEC>(row, c * 64 + lc * 4, dh);
+        }
+    }
+  };
+  constexpr uint64_t ALL = ~0ull;      // (lanes i and i + TK hold the same token)
+
+  char* vt = lds + wave * WAVE_BYTES;
+  int t0 = t_begin + wave * TK;
+  uint64_t next_valid = 0;
+  int entry, off;
+  if (t0 < t_end) {
+    look(t0, entry, off);
+    const int page = resolve(t0, entry, next_valid);
+    const int o = off;
+    look(t0 + 4 * TK, entry, off);
+    load(page, o);
+  }
+  for (; t0 < t_end; t0 += 4 * TK) {
+    const uint64_t valid = next_valid;
+    // ---- S^T = K . Q^T
+    floatx4_t s[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      s[f] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        uint4 kc = kr[f][c];
+        if (VEC && !EXACT) kc = keep_if(kc, c * (64 / (int)sizeof(T)) + g * PA<T>::E < dh);
+        if constexpr (BF) {
+          s[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kc), __builtin_bit_cast(bf16x8_t, qf[c]), s[f], 0, 0, 0);
+        } else {
+          const floatx4_t a = __builtin_bit_cast(floatx4_t, kc), q4 = __builtin_bit_cast(floatx4_t, qf[c]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], q4[j], s[f], 0, 0, 0);
+        }
       }
     }
-    __syncthreads();
-  }
-  l = wave_sum(l);
-  T* o = (T*)p.out + b * p.o_row + h * p.o_head;
+    // ---- this tile's V out of the load registers (rows that are no tokens as zeros: their weight is 0, but what lies there may be NaN)
+    if (valid != ALL) {
+      if constexpr (BF) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (c * 64 + lane < p.dh) o[c * 64 + lane] = from_f32<T>(l == 0.f ? 0.f : acc[c] / l);
-  if (p.lse && lane == 0) p.lse[(int64_t)b * p.H + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+        for (int i = 0; i < VC; ++i) vr[i] = keep_if(vr[i], (valid >> ((i * 64 + lane) / (DP / 8))) & 1);
+      } else {
+#pragma unroll
+        for (int i = 0; i < NF * 4 * (DP / 64); ++i) {
+          const int r = i / (DP / 64);
+          vr[i] = keep_if(vr[i], (valid >> ((r >> 2) * 16 + g * 4 + (r & 3))) & 1);
+        }
+      }
+    }
+    floatx4_t vcur[BF ? 1 : NF * 4 * (DP / 64 > 0 ? DP / 64 : 1)];
+    if constexpr (BF) {
+#pragma unroll
+      for (int i = 0; i < VC; ++i) {
+        const int r = (i * 64 + lane) / (DP / 8), col = (i * 64 + lane) % (DP / 8);
+        *reinterpret_cast<uint4*>(vt + r * RSV + col * 16) = vr[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NF * 4 * (DP / 64); ++i) vcur[i] = __builtin_bit_cast(floatx4_t, vr[i]);
+    }
+    // ---- the next tile's rows on their way, and the pages of the one behind it (past the end: rows and entries that exist, unused)
+    {
+      const int page = resolve(t0 + 4 * TK, entry, next_valid), o = off;
+      look(t0 + 8 * TK, entry, off);
+      load(page, o);
+    }
+    // ---- weights
+    float mx = -INFINITY;
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[f][r] = s[f][r] * p.scale_log2;
+        if (valid != ALL) s[f][r] = (valid >> (f * 16 + g * 4 + r)) & 1 ? s[f][r] : -INFINITY;
+        mx = fmaxf(mx, s[f][r]);
+      }
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float mn = fmaxf(m, mx), back = __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    float sum = 0.f;
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[f][r] = __builtin_amdgcn_exp2f(s[f][r] - mn);
+        sum += s[f][r];
+      }
+    l = l * back + sum;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) acc[i] *= back;
+    // ---- O^T += V^T . P^T
+    if constexpr (BF) {
+      static_assert(NF == 2 || !BF, "a bf16 product takes 32 tokens");
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      typedef short4_t __attribute__((address_space(3))) * lds_ptr_t;
+      union { uint32_t u[4]; bf16x8_t f; } w;
+      w.u[0] = pack_bf16x2(s[0][0], s[0][1]); w.u[1] = pack_bf16x2(s[0][2], s[0][3]);
+      w.u[2] = pack_bf16x2(s[NF - 1][0], s[NF - 1][1]); w.u[3] = pack_bf16x2(s[NF - 1][2], s[NF - 1][3]);
+      const char* base = vt + (g * 4 + (lc >> 2)) * RSV + (lc & 3) * 8;
+#pragma unroll
+      for (int i = 0; i < NA; ++i) {
+        union { short4_t h[2]; bf16x8_t f; } a;
+        a.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr_t)(base + i * 32));
+        a.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr_t)(base + i * 32 + 16 * RSV));
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.f, w.f, acc[i], 0, 0, 0);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    } else {
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int c = 0; c < DP / 64; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              acc[c * 4 + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vcur[(f * 4 + r) * (DP / 64) + c][j], s[f][r], acc[c * 4 + j], 0, 0, 0);
+    }
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  // ---- join the waves: O[wave][head][dim] in LDS
+  __syncthreads();
+  float* jo = reinterpret_cast<float*>(lds);
+  if (lane < 16) {
+    s_ml[0][wave][lc] = m;
+    s_ml[1][wave][lc] = l;
+  }
+  if (lc < nh) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        // f32: block c * 4 + j holds dims c * 64 + 4 * row + j
+        const int d = BF ? i * 16 + g * 4 + r : (i >> 2) * 64 + 4 * (g * 4 + r) + (i & 3);
+        jo[(wave * 16 + lc) * (DP + 4) + d] = acc[i][r];
+      }
+  }
+  __syncthreads();
+  for (int e = tid; e < nh * DP; e += 256) {
+    const int h = e / DP, d = e % DP;
+    if (d >= dh) continue;
+    const float mj = fmaxf(fmaxf(s_ml[0][0][h], s_ml[0][1][h]), fmaxf(s_ml[0][2][h], s_ml[0][3][h]));
+    float lj = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float c = __builtin_amdgcn_exp2f(s_ml[0][w][h] - mj);
+      lj += c * s_ml[1][w][h];
+      o += c * jo[(w * 16 + h) * (DP + 4) + d];
+    }
+    const int64_t row = (int64_t)b * p.H + h0 + h;
+    if (p.nsplit > 1) {
+      float* dst = p.part + (row * p.nsplit + split) * (p.dh + 2);
+      dst[d] = o;
+      if (d == 0) {
+        dst[p.dh] = mj;
+        dst[p.dh + 1] = lj;
+      }
+    } else {
+      ((T*)p.out)[b * p.o_row + (h0 + h) * p.o_head + d] = from_f32<T>(lj == 0.f ? 0.f : o / lj);
+      if (d == 0 && p.lse) p.lse[row] = lj == 0.f ? -INFINITY : (mj + log2f(lj)) * LN2;
+    }
+  }
+}
+
+// Joins the parts of a request: one workgroup per (request, head); wave w takes parts w, w + 4, ..., a lane the dims lane + 64 i.
+template <typename T>
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p) {
+  __shared__ float s_o[4][256], s_m[4], s_l[4];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int64_t row = blockIdx.x;
+  const int b = (int)(row / p.H), h = (int)(row - (int64_t)b * p.H);
+  const int len = min(max(p.lens[b], 0), p.max_pages * p.page_size);
+  const int part = part_tokens(len, p.nsplit), n = (int)(((int64_t)len + part - 1) / part);
+  const float* src = p.part + row * p.nsplit * (p.dh + 2);
+  float m = -3.402823466e38f;
+  for (int i = lane; i < n; i += 64) m = fmaxf(m, src[(int64_t)i * (p.dh + 2) + p.dh]);
+  m = wave_max(m);
+  float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = wave; i < n; i += 4) {
+    const float* s = src + (int64_t)i * (p.dh + 2);
+    const float c = __builtin_amdgcn_exp2f(s[p.dh] - m);
+    l += c * s[p.dh + 1];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k * 64 + lane < p.dh) o[k] += c * s[k * 64 + lane];
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) s_o[wave][k * 64 + lane] = o[k];
+  if (lane == 0) s_l[wave] = l;
+  __syncthreads();
+  l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+  if (tid < p.dh) {
+    const float v = (s_o[0][tid] + s_o[1][tid]) + (s_o[2][tid] + s_o[3][tid]);
+    ((T*)p.out)[b * p.o_row + h * p.o_head + tid] = from_f32<T>(l == 0.f ? 0.f : v / l);
+  }
+  if (tid == 0 && p.lse) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+template <typename T, int DP, int NF>
+void paged_attn_launch(const PagedAttnParams& p, bool vec, unsigned grid, hipStream_t st) {
+  if (vec && p.dh == DP) paged_attn_kernel<T, DP, NF, true, true><<<grid, 256, 0, st>>>(p);
+  else if (vec) paged_attn_kernel<T, DP, NF, true, false><<<grid, 256, 0, st>>>(p);
+  else paged_attn_kernel<T, DP, NF, false, false><<<grid, 256, 0, st>>>(p);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -296,7 +586,7 @@ extern "C" int nst_paged_plan(const int32_t* cached_lens, const int32_t* new_len
   NST_CHECK_ARG(B >= 0 && max_pages > 0 && page_size > 0 && n_free >= 0 && max_tokens >= 0,
                 "nst_paged_plan: B=%d max_pages=%d page_size=%d n_free=%d max_tokens=%lld", B, max_pages, page_size, n_free,
                 (long long)max_tokens);
-  NST_CHECK_ARG((int64_t)max_pages * page_size <= 0x7fffffffLL, "nst_paged_plan: %d pages of %d tokens pass 2^31 - 1 positions", max_pages,
+  NST_CHECK_ARG((int64_t)max_pages * page_size <= MAX_POSITIONS, "nst_paged_plan: %d pages of %d tokens pass 2^30 positions", max_pages,
                 page_size);
   NST_CHECK_ARG(cursor_in && cu_new && cursor_out && (slots || max_tokens == 0) && (free_pages || n_free == 0),
                 "nst_paged_plan: NULL pointer");
@@ -359,15 +649,30 @@ static int paged_attention_check(const NstPagedAttnDesc* d) {
   NST_CHECK_ARG(pl.page_size > 0 && pl.num_pages >= 0 && d->max_pages > 0 && d->table_stride >= d->max_pages && d->max_len >= 0,
                 "nst_paged_attention: page_size=%d num_pages=%d max_pages=%d table stride %lld max_len=%d", pl.page_size, pl.num_pages,
                 d->max_pages, (long long)d->table_stride, d->max_len);
-  NST_CHECK_ARG((int64_t)d->max_pages * pl.page_size <= 0x7fffffffLL, "nst_paged_attention: %d pages of %d tokens pass 2^31 - 1 positions",
+  NST_CHECK_ARG((int64_t)d->max_pages * pl.page_size <= MAX_POSITIONS, "nst_paged_attention: %d pages of %d tokens pass 2^30 positions",
                 d->max_pages, pl.page_size);
+  const int64_t rows[4] = {pl.k_page_stride, pl.k_token_stride, pl.v_page_stride, pl.v_token_stride};
+  for (int i = 0; i < 4; ++i)
+    NST_CHECK_ARG(rows[i] >= 0 && rows[i] <= 0x7fffffffLL, "nst_paged_attention: page or token stride %lld (0 .. 2^31 - 1 elements)",
+                  (long long)rows[i]);
   NST_CHECK_ARG((int64_t)d->B * d->H <= 0x7fffffffLL, "nst_paged_attention: %d x %d rows", d->B, d->H);
   return NST_OK;
 }
 
+// How many parts a request is cut into at most.  Enough workgroups for every CU to hold several, but no part below MIN_PART tokens.
+static int paged_attention_splits(const NstPagedAttnDesc* d) {
+  const int64_t cap = (int64_t)d->max_pages * d->pool.page_size, bound = d->max_len > 0 && d->max_len < cap ? d->max_len : cap;
+  const int64_t units = (int64_t)d->B * d->Hkv * ((d->H / d->Hkv + 15) / 16);
+  const int64_t most = (bound + MIN_PART - 1) / MIN_PART, want = (2048 + units - 1) / units;
+  const int64_t n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n);
+}
+
 extern "C" int64_t nst_paged_attention_workspace_bytes(const NstPagedAttnDesc* d) {
   const int rc = paged_attention_check(d);
-  return rc != NST_OK ? rc : 0;
+  if (rc != NST_OK) return rc;
+  const int n = d->B > 0 ? paged_attention_splits(d) : 1;
+  return n > 1 ? (int64_t)d->B * d->H * n * (d->dh + 2) * (int64_t)sizeof(float) : 0;
 }
 
 extern "C" int nst_paged_attention(const NstPagedAttnDesc* d, const void* q, const void* k_pool, const void* v_pool,
@@ -377,14 +682,62 @@ extern "C" int nst_paged_attention(const NstPagedAttnDesc* d, const void* q, con
   if (rc != NST_OK) return rc;
   if (d->B == 0) return NST_OK;
   NST_CHECK_ARG(q && block_table && seq_lens && out && ((k_pool && v_pool) || d->pool.num_pages == 0), "nst_paged_attention: NULL pointer");
-  (void)workspace; (void)workspace_bytes;
   const NstPagedPool& pl = d->pool;
-  PagedAttnParams p = {q, k_pool, v_pool, out, lse, block_table, seq_lens, d->B, d->H, d->Hkv, d->dh, pl.page_size, pl.num_pages,
-                       d->max_pages, d->q_row_stride, d->q_head_stride, d->o_row_stride, d->o_head_stride, d->table_stride,
-                       pl.k_page_stride, pl.k_token_stride, pl.k_head_stride, pl.v_page_stride, pl.v_token_stride, pl.v_head_stride,
-                       d->scale};
-  if (pl.dtype == NST_BF16) paged_attn_kernel<bf16_t><<<d->B * d->H, 64, 0, (hipStream_t)stream>>>(p);
-  else paged_attn_kernel<float><<<d->B * d->H, 64, 0, (hipStream_t)stream>>>(p);
+  PagedAttnParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = (const char*)q; p.k = (const char*)k_pool; p.v = (const char*)v_pool; p.out = (char*)out; p.lse = lse;
+  p.table = block_table; p.lens = seq_lens;
+  p.B = d->B; p.H = d->H; p.Hkv = d->Hkv; p.dh = d->dh;
+  p.page_size = pl.page_size; p.num_pages = pl.num_pages; p.max_pages = d->max_pages;
+  p.q_row = d->q_row_stride; p.q_head = d->q_head_stride; p.o_row = d->o_row_stride; p.o_head = d->o_head_stride;
+  p.table_stride = d->table_stride;
+  if (pl.num_pages > 0) {
+    p.k_page = (uint32_t)pl.k_page_stride; p.k_tok = (uint32_t)pl.k_token_stride; p.k_head = pl.k_head_stride;
+    p.v_page = (uint32_t)pl.v_page_stride; p.v_tok = (uint32_t)pl.v_token_stride; p.v_head = pl.v_head_stride;
+  } else {
+    p.k = p.v = p.q;       // no page exists: every row the kernel touches (and ignores) is the first row of q
+  }
+  p.scale_log2 = d->scale * LOG2E;
+  p.qchunks = (d->H / d->Hkv + 15) / 16;
+  p.nsplit = paged_attention_splits(d);
+  // t / d by multiplication: with s = ceil(log2 d) and magic = floor(2^(31 + s) / d) + 1 the quotient is exact below 2^31
+  int s = 0;
+  while ((1LL << s) < pl.page_size) ++s;
+  if (s > 0) {
+    p.div_magic = (uint32_t)((1ULL << (31 + s)) / (uint64_t)pl.page_size + 1);
+    p.div_shift = s - 1;
+  }
+  if (p.nsplit > 1) {
+    const int64_t need = (int64_t)d->B * d->H * p.nsplit * (d->dh + 2) * (int64_t)sizeof(float);
+    if (!workspace || workspace_bytes < need || !nst_aligned16(workspace)) {
+      nst_set_error("nst_paged_attention: workspace of %lld bytes, needs %lld (16-byte aligned)", (long long)workspace_bytes, (long long)need);
+      return NST_ERR_WORKSPACE;
+    }
+    p.part = (float*)workspace;
+  }
+  const int64_t blocks = (int64_t)d->B * d->Hkv * p.qchunks * p.nsplit;
+  NST_CHECK_ARG(blocks <= 0x7fffffffLL, "nst_paged_attention: %lld workgroups", (long long)blocks);
+  const int es = nst_dtype_size(pl.dtype);
+  bool vec = nst_aligned16(q) && nst_aligned16(p.k) && nst_aligned16(p.v) && (d->dh * es) % 16 == 0;
+  const int64_t strides[8] = {p.q_row, p.q_head, p.k_page, p.k_tok, p.k_head, p.v_page, p.v_tok, p.v_head};
+  for (int i = 0; i < 8; ++i) vec = vec && (strides[i] * es) % 16 == 0;
+  hipStream_t st = (hipStream_t)stream;
+  const unsigned grid = (unsigned)blocks;
+  if (pl.dtype == NST_BF16) {
+    if (d->dh <= 32) paged_attn_launch<bf16_t, 32, 2>(p, vec, grid, st);
+    else if (d->dh <= 64) paged_attn_launch<bf16_t, 64, 2>(p, vec, grid, st);
+    else if (d->dh <= 128) paged_attn_launch<bf16_t, 128, 2>(p, vec, grid, st);
+    else paged_attn_launch<bf16_t, 256, 2>(p, vec, grid, st);
+  } else {
+    if (d->dh <= 64) paged_attn_launch<float, 64, 2>(p, vec, grid, st);
+    else if (d->dh <= 128) paged_attn_launch<float, 128, 2>(p, vec, grid, st);
+    else paged_attn_launch<float, 256, 1>(p, vec, grid, st);
+  }
+  if (p.nsplit > 1) {
+    NST_CHECK_LAUNCH("nst_paged_attention");
+    if (pl.dtype == NST_BF16) paged_attn_join_kernel<bf16_t><<<d->B * d->H, 256, 0, st>>>(p);
+    else paged_attn_join_kernel<float><<<d->B * d->H, 256, 0, st>>>(p);
+  }
   NST_CHECK_LAUNCH("nst_paged_attention");
   return NST_OK;
 }
@@ -396,7 +749,7 @@ extern "C" int nst_paged_reorder(void* pool, int planes, int64_t plane_stride, i
   NST_CHECK_ARG(planes > 0 && planes <= 65535 && num_pages >= 0 && page_size > 0 && token_bytes > 0 && max_pages > 0 && rows >= 0,
                 "nst_paged_reorder: planes=%d num_pages=%d page_size=%d token_bytes=%lld max_pages=%d rows=%d", planes, num_pages,
                 page_size, (long long)token_bytes, max_pages, rows);
-  NST_CHECK_ARG((int64_t)max_pages * page_size <= 0x7fffffffLL, "nst_paged_reorder: %d pages of %d tokens pass 2^31 - 1 positions", max_pages,
+  NST_CHECK_ARG((int64_t)max_pages * page_size <= MAX_POSITIONS, "nst_paged_reorder: %d pages of %d tokens pass 2^30 positions", max_pages,
                 page_size);
   NST_CHECK_ARG(page_stride >= token_bytes * page_size || num_pages <= 1, "nst_paged_reorder: pages of %lld bytes %lld bytes apart",
                 (long long)(token_bytes * page_size), (long long)page_stride);

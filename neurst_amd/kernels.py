@@ -741,11 +741,6 @@ def attention_bwd(q, k, v, out, dout, lse, dq, dk, dv, H, dh, key_bias=None, cau
 
 
 # ------------------------------------------------------------------------------------------------ paged key / value caches
-def _require(ok, message):
-    if not ok:
-        raise ValueError(message)
-
-
 def _on_device(what, *tensors):
     """Every operand lives on the CURRENT device: the launch goes to its current stream."""
     for t in tensors:
@@ -758,24 +753,25 @@ def _on_device(what, *tensors):
 
 
 def _index_vector(what, name, t, dtype, n=None):
-    _require(t.dim() == 1 and t.dtype == dtype and (n is None or t.shape[0] == n) and (t.stride(0) == 1 or t.shape[0] <= 1),
-             f"{what}: {name} must be a dense {dtype} vector" + ("" if n is None else f" of {n}") + f", got {t.dtype} {tuple(t.shape)}")
+    if not (t.dim() == 1 and t.dtype == dtype and (n is None or t.shape[0] == n) and (t.stride(0) == 1 or t.shape[0] <= 1)):
+        raise ValueError(f"{what}: {name} must be a dense {dtype} vector" + ("" if n is None else f" of {n}") + f", got {t.dtype} {tuple(t.shape)}")
 
 
 def _block_table(what, t, rows):
-    _require(t.dim() == 2 and t.dtype == torch.int32 and t.shape[0] == rows and t.shape[1] > 0 and (t.stride(1) == 1 or t.shape[1] == 1),
-             f"{what}: block_table must be int32 [{rows}, pages] with dense rows, got {t.dtype} {tuple(t.shape)}")
+    if not (t.dim() == 2 and t.dtype == torch.int32 and t.shape[0] == rows and t.shape[1] > 0 and (t.stride(1) == 1 or t.shape[1] == 1)):
+        raise ValueError(f"{what}: block_table must be int32 [{rows}, pages] with dense rows, got {t.dtype} {tuple(t.shape)}")
     stride = t.stride(0) if rows > 1 else t.shape[1]
-    _require(stride >= t.shape[1], f"{what}: rows of block_table overlap")
+    if not (stride >= t.shape[1]):
+        raise ValueError(f"{what}: rows of block_table overlap")
     return stride
 
 
 def _paged_pool(what, k_pool, v_pool):
     """[pages, page_size, kv_heads, dh] views (any strides, dense heads) -> NstPagedPool."""
-    _require(k_pool.dim() == 4 and k_pool.shape == v_pool.shape and k_pool.dtype == v_pool.dtype and min(k_pool.shape[1:]) > 0,
-             f"{what}: k_pool and v_pool must be [pages, page_size, kv_heads, dh] of one type, got {k_pool.dtype} {tuple(k_pool.shape)} and "
-             f"{v_pool.dtype} {tuple(v_pool.shape)}")
-    _require(k_pool.shape[3] == 1 or (k_pool.stride(3) == 1 and v_pool.stride(3) == 1), f"{what}: the elements of a head must be dense")
+    if not (k_pool.dim() == 4 and k_pool.shape == v_pool.shape and k_pool.dtype == v_pool.dtype and min(k_pool.shape[1:]) > 0):
+        raise ValueError(f"{what}: k_pool and v_pool must be [pages, page_size, kv_heads, dh] of one type, got {k_pool.dtype} {tuple(k_pool.shape)} and " f"{v_pool.dtype} {tuple(v_pool.shape)}")
+    if not (k_pool.shape[3] == 1 or (k_pool.stride(3) == 1 and v_pool.stride(3) == 1)):
+        raise ValueError(f"{what}: the elements of a head must be dense")
     return NstPagedPool(k_pool.shape[0], k_pool.shape[1], _dt(k_pool), 0, k_pool.stride(0), k_pool.stride(1), k_pool.stride(2),
                         v_pool.stride(0), v_pool.stride(1), v_pool.stride(2))
 
@@ -805,9 +801,10 @@ def paged_append(k, v, k_pool, v_pool, slots):
     """Rows k, v [tokens, kv_heads, dh] into their slots of the pools [pages, page_size, kv_heads, dh] (in place); slots int64 [tokens], a
     slot outside the pools is skipped, no slot may appear twice."""
     pool = _paged_pool("paged_append", k_pool, v_pool)
-    _require(k.dim() == 3 and k.shape == v.shape and k.shape[1:] == k_pool.shape[2:] and k.dtype == v.dtype == k_pool.dtype,
-             f"paged_append: rows {k.dtype} {tuple(k.shape)} / {v.dtype} {tuple(v.shape)} for pools {k_pool.dtype} {tuple(k_pool.shape)}")
-    _require(k.shape[2] == 1 or (k.stride(2) == 1 and v.stride(2) == 1), "paged_append: the elements of a head must be dense")
+    if not (k.dim() == 3 and k.shape == v.shape and k.shape[1:] == k_pool.shape[2:] and k.dtype == v.dtype == k_pool.dtype):
+        raise ValueError(f"paged_append: rows {k.dtype} {tuple(k.shape)} / {v.dtype} {tuple(v.shape)} for pools {k_pool.dtype} {tuple(k_pool.shape)}")
+    if not (k.shape[2] == 1 or (k.stride(2) == 1 and v.stride(2) == 1)):
+        raise ValueError("paged_append: the elements of a head must be dense")
     _index_vector("paged_append", "slots", slots, torch.int64, k.shape[0])
     _on_device("paged_append", k, v, k_pool, v_pool, slots)
     check(lib.nst_paged_append(_p(k), _p(v), k.shape[0], k.shape[1], k.shape[2], k.stride(0), k.stride(1), v.stride(0), v.stride(1),
@@ -820,8 +817,8 @@ def paged_attention(q, k_pool, v_pool, block_table, seq_lens, scale=None, max_le
     scale: dh^-0.5 by default.  max_len: a bound of seq_lens the host knows; it chooses how the work is split, never the result's
     extent."""
     pool = _paged_pool("paged_attention", k_pool, v_pool)
-    _require(q.dim() == 3 and q.dtype == k_pool.dtype and q.shape[2] == k_pool.shape[3] and q.shape[1] > 0
-             and (q.shape[2] == 1 or q.stride(2) == 1), f"paged_attention: q {q.dtype} {tuple(q.shape)} for pools {k_pool.dtype} {tuple(k_pool.shape)}")
+    if not (q.dim() == 3 and q.dtype == k_pool.dtype and q.shape[2] == k_pool.shape[3] and q.shape[1] > 0 and (q.shape[2] == 1 or q.stride(2) == 1)):
+        raise ValueError(f"paged_attention: q {q.dtype} {tuple(q.shape)} for pools {k_pool.dtype} {tuple(k_pool.shape)}")
     B, H, dh = q.shape
     _index_vector("paged_attention", "seq_lens", seq_lens, torch.int32, B)
     stride = _block_table("paged_attention", block_table, B)
@@ -845,9 +842,8 @@ def paged_reorder(pool, block_table, seq_lens, parents, spare):
     """Re-ordering behind a beam-search step (nst_paged_reorder): row r continues row parents[r] (int64), which is as long.  pool [planes,
     pages, page_size, width]: the partly filled pages are copied in place, full pages are shared; spare [R] int32: one free page
     per row.  Returns the new (block_table, spare)."""
-    _require(pool.dim() == 4 and min(pool.shape[0], pool.shape[2], pool.shape[3]) > 0 and (pool.shape[3] == 1 or pool.stride(3) == 1)
-             and (pool.shape[2] == 1 or pool.stride(2) == pool.shape[3]),
-             f"paged_reorder: pool must be [planes, pages, page_size, width] with dense pages, got {tuple(pool.shape)} / {pool.stride()}")
+    if not (pool.dim() == 4 and min(pool.shape[0], pool.shape[2], pool.shape[3]) > 0 and (pool.shape[3] == 1 or pool.stride(3) == 1) and (pool.shape[2] == 1 or pool.stride(2) == pool.shape[3])):
+        raise ValueError(f"paged_reorder: pool must be [planes, pages, page_size, width] with dense pages, got {tuple(pool.shape)} / {pool.stride()}")
     R = block_table.shape[0] if block_table.dim() == 2 else -1
     stride = _block_table("paged_reorder", block_table, R)
     _index_vector("paged_reorder", "seq_lens", seq_lens, torch.int32, R)
@@ -869,8 +865,8 @@ def token_logprobs(logits, tokens, top_n=0):
     """logits [rows, V], tokens [rows] int64 -> (logp, entropy, lse [rows] f32, top_logp [rows, top_n] f32, top_ids [rows, top_n] int64):
     the log probability of the given token (0 for a token outside [0, V)), the entropy, the log-sum-exp and the top_n <= 64 likeliest
     tokens of every row, equal logits by the lower id (nst_token_logprobs_fwd)."""
-    _require(logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1),
-             f"token_logprobs: logits must be [rows, vocabulary] with dense rows, got {tuple(logits.shape)} / {logits.stride()}")
+    if not (logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1)):
+        raise ValueError(f"token_logprobs: logits must be [rows, vocabulary] with dense rows, got {tuple(logits.shape)} / {logits.stride()}")
     rows, V = logits.shape
     _index_vector("token_logprobs", "tokens", tokens, torch.int64, rows)
     _on_device("token_logprobs", logits, tokens)
@@ -891,8 +887,8 @@ def token_logprobs(logits, tokens, top_n=0):
 def token_logprobs_bwd(logits, tokens, lse, entropy, dlogp, dentropy=None, out=None):
     """d(logits) from d(logp) and d(entropy) (either None: zero), with the lse and entropy that token_logprobs returned
     (nst_token_logprobs_bwd).  out: where to write it; may be logits itself."""
-    _require(logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1),
-             f"token_logprobs_bwd: logits must be [rows, vocabulary] with dense rows, got {tuple(logits.shape)} / {logits.stride()}")
+    if not (logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1)):
+        raise ValueError(f"token_logprobs_bwd: logits must be [rows, vocabulary] with dense rows, got {tuple(logits.shape)} / {logits.stride()}")
     rows, V = logits.shape
     _index_vector("token_logprobs_bwd", "tokens", tokens, torch.int64, rows)
     for name, t in (("lse", lse), ("entropy", entropy), ("dlogp", dlogp), ("dentropy", dentropy)):
@@ -900,8 +896,8 @@ def token_logprobs_bwd(logits, tokens, lse, entropy, dlogp, dentropy=None, out=N
             _index_vector("token_logprobs_bwd", name, t, torch.float32, rows)
     if out is None:
         out = torch.empty(rows, V, dtype=logits.dtype, device=logits.device)
-    _require(out.shape == logits.shape and out.dtype == logits.dtype and (out.stride(1) == 1 or V == 1),
-             f"token_logprobs_bwd: out {out.dtype} {tuple(out.shape)} for logits {logits.dtype} {tuple(logits.shape)}")
+    if not (out.shape == logits.shape and out.dtype == logits.dtype and (out.stride(1) == 1 or V == 1)):
+        raise ValueError(f"token_logprobs_bwd: out {out.dtype} {tuple(out.shape)} for logits {logits.dtype} {tuple(logits.shape)}")
     _on_device("token_logprobs_bwd", logits, tokens, lse, entropy, dlogp, dentropy, out)
     check(lib.nst_token_logprobs_bwd(_p(logits), _p(tokens), _p(lse), _p(entropy), _p(dlogp), _p(dentropy), _p(out), rows, V,
                                      logits.stride(0), out.stride(0), _dt(logits), _stream()), "token_logprobs_bwd")

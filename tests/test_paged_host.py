@@ -31,7 +31,7 @@ def plan(B=1, stride=4, max_pages=4, n_free=1, page_size=4, max_tokens=1, cursor
 
 @pytest.mark.parametrize("kw,text", [
     (dict(B=-1), "B=-1"), (dict(page_size=0), "page_size=0"), (dict(max_pages=0), "max_pages=0"), (dict(max_tokens=-1), "max_tokens=-1"),
-    (dict(stride=3), "stride 3"), (dict(max_pages=1 << 20, stride=1 << 20, page_size=1 << 12), "2^31"), (dict(slots=None), "NULL"),
+    (dict(stride=3), "stride 3"), (dict(max_pages=1 << 20, stride=1 << 20, page_size=1 << 12), "2^30"), (dict(slots=None), "NULL"),
     (dict(free=None), "NULL"), (dict(cached=None), "NULL"), (dict(cursor_out=4096), "overlap"), (dict(seq=4096), "overlap")])
 def test_plan_refuses(kw, text):
     assert plan(**kw) == ARG and text in message()
@@ -55,7 +55,7 @@ def attn(**kw):
 @pytest.mark.parametrize("kw,text", [
     (dict(H=3), "3 heads over 2"), (dict(Hkv=0), "0 key"), (dict(dh=257), "head size 257"), (dict(dh=0), "head size 0"), (dict(dtype=2), "dtype 2"),
     (dict(page_size=0), "page_size=0"), (dict(table_stride=3), "stride 3"), (dict(max_len=-1), "max_len=-1"), (dict(q=None), "NULL"),
-    (dict(k=None), "NULL"), (dict(out=None), "NULL"), (dict(lens=None), "NULL"), (dict(max_pages=1 << 28, table_stride=1 << 28), "2^31"),
+    (dict(k=None), "NULL"), (dict(out=None), "NULL"), (dict(lens=None), "NULL"), (dict(max_pages=1 << 28, table_stride=1 << 28), "2^30"),
     (dict(B=1 << 30), "rows")])
 def test_attention_refuses(kw, text):
     rc, d = attn(**kw)
