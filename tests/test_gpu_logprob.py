@@ -161,7 +161,10 @@ def assert_backward(K, x, tokens, a, b, out=None):
     rel = U * (x0.abs() + l64.abs() + 3 * safe.abs() + 16)
     mag = p * (a64.abs() + b64.abs() * (safe.abs() + h64.abs() + 1))
     half = 2.0 ** -8 if x.dtype == torch.bfloat16 else U
-    tol = 4 * rel * mag + 2 * U * hot * a64.abs() + half * want.abs() + 1e-37      # (p below 2^-126 is flushed)
+    # a probability below 2^-126 is flushed to 0, which is off by less than 2^-126, and that factor times |a + b (log p + H)| in the
+    # product; a product that falls below 2^-126 itself is flushed as well: another 2^-126
+    flushed = 2.0 ** -126 * (1 + a64.abs() + b64.abs() * (safe.abs() + h64.abs()))
+    tol = 4 * rel * mag + 2 * U * hot * a64.abs() + half * want.abs() + flushed
     err = (g.cpu().double() - want).abs()
     assert (err <= tol).all(), float((err / tol).max())
     return g
