@@ -205,6 +205,7 @@ __global__ void __launch_bounds__(256) token_logprobs_kernel(LogprobParams p) {
     for (int i = tid; i < count; i += 256) {
       const uint64_t key = cand[i];
       int rank = 0;
+#pragma unroll 8
       for (int j = 0; j < count; ++j) rank += cand[j] > key;
       if (rank < want) emit(rank, key);
     }
@@ -296,12 +297,13 @@ __global__ void __launch_bounds__(256) token_logprobs_kernel(LogprobParams p) {
   }
 }
 
-// Joins the parts of a row: one wave, lane i has part i.  Alternatives: only the top_n parts with the largest heads can hold any, and of
+// Joins the parts of a row: lane i of every wave has part i (four waves only so that the lists arrive at once).  Alternatives: only the top_n parts with the largest heads can hold any, and of
 // those only what is not below the smallest of these heads.
 template <typename T>
-__global__ void __launch_bounds__(64) token_logprobs_join_kernel(LogprobParams p) {
+__global__ void __launch_bounds__(256) token_logprobs_join_kernel(LogprobParams p) {
   extern __shared__ uint64_t lists[];                  // [nparts][top_n], then the lists' heads and, in their place, the candidates
-  const int lane = threadIdx.x, np = p.nparts, n = p.top_n;
+  __shared__ int s_count;
+  const int tid = threadIdx.x, lane = tid & 63, np = p.nparts, n = p.top_n;
   const int64_t row = blockIdx.x;
   const float* st = p.stats + row * np * 4;
   float m = -INFINITY, s = 0.f, t = 0.f;
@@ -309,40 +311,53 @@ __global__ void __launch_bounds__(64) token_logprobs_join_kernel(LogprobParams p
     const float4 q = reinterpret_cast<const float4*>(st)[lane];
     m = q.x; s = q.y; t = q.z;
   }
-  for (int i = lane; i < np * n; i += 64) lists[i] = p.keys[row * np * n + i];
+  uint64_t *heads = lists + np * n, *cand = heads;
+  {
+    const uint64_t* src = p.keys + row * np * n;
+    const uint64_t head = n > 0 && lane < np ? src[lane * n] : 0;
+    uint64_t v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = i * 256 + tid < np * n ? src[i * 256 + tid] : 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i * 256 + tid < np * n) lists[i * 256 + tid] = v[i];
+    if (tid < MAX_PARTS) heads[tid] = head;
+  }
   const float M = wave_max(m), mu = M == -INFINITY ? 0.f : M;
   const float d = m - mu, c = __builtin_amdgcn_exp2f(d * LOG2E);
   t = wave_sum(c * fmaf(fmaxf(d, LOWEST), s, t));
   s = wave_sum(c * s);
   const float log_s = M == -INFINITY ? NAN : logf(s), lse = M + log_s;
-  if (lane == 0) write_row<T>(p, row, lse, log_s, t / s);
+  if (tid == 0) write_row<T>(p, row, lse, log_s, t / s);
   if (n == 0) return;
   __syncthreads();
-  uint64_t *heads = lists + np * n, *cand = heads;
-  const uint64_t head = lane < np ? lists[lane * n] : 0;
-  heads[lane] = head;
-  __syncthreads();
+  const uint64_t head = heads[lane];
   int rank = 0;
+#pragma unroll 8
   for (int j = 0; j < np; ++j) rank += heads[j] > head;
-  // (heads differ: a key holds its index.  Parts without any element left do not occur: a part is never empty)
+  // (heads differ: a key holds its index, and no part is empty)
   const uint64_t nth = __ballot(lane < np && rank == n - 1);
   const uint64_t tau = nth ? heads[__ffsll((unsigned long long)nth) - 1] : 1;
-  int cnt = 0;
-  if (lane < np && head >= tau)
-    while (cnt < n && lists[lane * n + cnt] >= tau) ++cnt;
-  int incl = cnt;
+  __syncthreads();                                      // the candidates take the heads' place
+  if (tid < 64) {
+    int cnt = 0;
+    if (lane < np && head >= tau)
+      while (cnt < n && lists[lane * n + cnt] >= tau) ++cnt;
+    int incl = cnt;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int up = __shfl_up(incl, o, 64);
-    if (lane >= o) incl += up;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += up;
+    }
+    for (int k = 0; k < cnt; ++k) cand[incl - cnt + k] = lists[lane * n + k];
+    if (lane == 63) s_count = incl;
   }
   __syncthreads();
-  for (int k = 0; k < cnt; ++k) cand[incl - cnt + k] = lists[lane * n + k];
-  const int count = __shfl(incl, 63, 64);
-  __syncthreads();
-  for (int i = lane; i < count; i += 64) {
+  const int count = s_count;
+  for (int i = tid; i < count; i += 256) {
     const uint64_t key = cand[i];
     int r = 0;
+#pragma unroll 8
     for (int j = 0; j < count; ++j) r += cand[j] > key;
     if (r < n) write_top(p, row, r, key, lse);
   }
@@ -395,11 +410,12 @@ __global__ void __launch_bounds__(256) token_logprobs_bwd_kernel(const T* logits
 struct LogprobSplit {
   int nparts, part, pieces;     // pieces: of a thread
 };
-// Rows of up to 16384 elements stay whole when there are rows enough to fill the chip; few rows are cut into at most 64 parts of at least 1024
-// elements, so that a short batch over a large vocabulary is read by every CU.
+// Rows of up to 16384 elements stay whole when there are rows enough for every second CU: cutting 128 rows of 8008 in four measured
+// SPLIT_STEP.  Fewer rows are cut into at most 64 parts of at least 1024 elements, so that a short batch over a large vocabulary is
+// read by every CU.
 static LogprobSplit logprob_split(int64_t rows, int V, int dtype) {
   const int E = dtype == NST_BF16 ? 8 : 4, most = 16384;
-  int64_t want = rows > 0 ? (512 + rows - 1) / rows : 1;
+  int64_t want = rows >= 128 ? 1 : rows > 0 ? (256 + rows - 1) / rows : 1;
   if (want > (V + 1023) / 1024) want = (V + 1023) / 1024;
   if (want < (V + most - 1) / most) want = (V + most - 1) / most;
   if (want > MAX_PARTS) want = MAX_PARTS;
@@ -463,8 +479,8 @@ extern "C" int nst_token_logprobs_fwd(const void* logits, const int64_t* tokens,
   if (sp.nparts > 1) {
     NST_CHECK_LAUNCH("nst_token_logprobs_fwd");
     const size_t held = (size_t)sp.nparts * top_n, lds = sizeof(uint64_t) * (held + (held > MAX_PARTS ? held : MAX_PARTS));      // at most 64 KiB
-    if (dtype == NST_BF16) token_logprobs_join_kernel<bf16_t><<<(unsigned)rows, 64, lds, st>>>(p);
-    else token_logprobs_join_kernel<float><<<(unsigned)rows, 64, lds, st>>>(p);
+    if (dtype == NST_BF16) token_logprobs_join_kernel<bf16_t><<<(unsigned)rows, 256, lds, st>>>(p);
+    else token_logprobs_join_kernel<float><<<(unsigned)rows, 256, lds, st>>>(p);
   }
   NST_CHECK_LAUNCH("nst_token_logprobs_fwd");
   return NST_OK;

@@ -14,21 +14,41 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 constexpr int64_t MAX_POSITIONS = 1 << 30;     // of one request: position arithmetic, a tile or two past the end included, stays in 32 bits
 
+// t / d for 0 <= t < 2^31 by one multiplication: with s = ceil(log2 d) and magic = floor(2^(31 + s) / d) + 1 the error of t * magic / 2^(31 + s)
+// stays below 1 / d, so the quotient is exact.  magic == 0: d == 1.
+struct FastDiv {
+  uint32_t d, magic;
+  int shift;
+  __device__ __forceinline__ uint32_t div(uint32_t t) const { return magic ? __umulhi(t, magic) >> shift : t; }
+  __device__ __forceinline__ uint32_t up(uint32_t t) const { return div(t + d - 1); }      // (t + d - 1 < 2^31 too)
+};
+FastDiv fast_div(int d) {
+  FastDiv f = {(uint32_t)d, 0, 0};
+  int s = 0;
+  while ((1LL << s) < d) ++s;
+  if (s > 0) {
+    f.magic = (uint32_t)((1ULL << (31 + s)) / (uint64_t)d + 1);
+    f.shift = s - 1;
+  }
+  return f;
+}
+
 // ---------------------------------------------------------------------------------------------
 // plan
 // ---------------------------------------------------------------------------------------------
 struct PlanParams {
   const int32_t *cached, *fresh;
-  int B, page_size, max_pages;
+  int B, max_pages;
+  FastDiv page;
   int32_t* table;
   int64_t table_stride;
   const int32_t* free_pages;
   int n_free;
   const int32_t* cursor_in;
   int64_t* slots;
-  int64_t max_tokens;
+  int max_tokens;
   int32_t *seq_lens, *cu_new, *cursor_out;
-  int per_group;   // requests of one workgroup (<= 256)
+  int per_group;   // requests of one workgroup (<= 64)
 };
 
 struct PlanRequest {
@@ -36,63 +56,77 @@ struct PlanRequest {
 };
 __device__ __forceinline__ PlanRequest plan_request(const PlanParams& p, int b) {
   PlanRequest r;
-  const int64_t cap = (int64_t)p.max_pages * p.page_size;
-  const int64_t c = max(p.cached[b], 0), n = max(p.fresh[b], 0);
-  r.cached = (int)(c < cap ? c : cap);
-  r.fresh = (int)n;
-  const int64_t end = r.cached + n < cap ? r.cached + n : cap;
-  r.held = (int)((r.cached + p.page_size - 1) / p.page_size);
-  r.need = (int)((end + p.page_size - 1) / p.page_size) - r.held;
+  const int cap = p.max_pages * (int)p.page.d;             // <= 2^30
+  r.cached = min(max(p.cached[b], 0), cap);
+  r.fresh = max(p.fresh[b], 0);
+  r.held = (int)p.page.up(r.cached);
+  r.need = (int)p.page.up(r.cached + min(r.fresh, cap - r.cached)) - r.held;
   return r;
 }
+__device__ __forceinline__ int64_t wave_sum_i64(int64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
 
-// Every workgroup sums the wishes of the requests in front of its own (B * 8 bytes from the cache: cheaper than a launch that
-// scans them first) and scans its own; then its threads walk the group's pages and tokens as one flat range, so that one long
+// Every workgroup sums the wishes of the requests in front of its own (8 bytes each, from the cache: cheaper than a launch that scans
+// them first) while its first wave scans its own; then its threads walk the group's pages and tokens as one flat range, so that one long
 // prompt among many short requests keeps all of them busy.  blockIdx.y splits the tokens of a group further.
+// Bound by latency: two reads from the cache and two barriers before the first slot is known.
+// 128 requests of one token: GPU_PLAN_STEP us; 2047 prompts, 1.05 M tokens: GPU_PLAN_PREFILL us.
 __global__ void __launch_bounds__(256) paged_plan_kernel(PlanParams p) {
-  __shared__ int64_t red[2][256];
-  __shared__ int64_t tok_off[257], page_off[257];
-  __shared__ int s_cached[256], s_held[256];
-  const int tid = threadIdx.x;
+  __shared__ int64_t red[2][4];
+  __shared__ int tok_off[65], page_off[65];                // saturated at 2^31 - 1: nothing behind that is used
+  __shared__ int s_cached[64], s_held[64];
+  const int tid = threadIdx.x, lane = tid & 63;
   const int b0 = blockIdx.x * p.per_group, nb = min(p.per_group, p.B - b0);
+  const int cursor = max(*p.cursor_in, 0);
   int64_t tok = 0, pages = 0;
-  for (int b = tid; b < b0; b += 256) {
+  int b = tid;
+  for (; b + 768 < b0; b += 1024) {                        // (four at a time: the reads are independent)
+    PlanRequest r[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r[k] = plan_request(p, b + k * 256);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      tok += r[k].fresh;
+      pages += r[k].need;
+    }
+  }
+  for (; b < b0; b += 256) {
     const PlanRequest r = plan_request(p, b);
     tok += r.fresh;
     pages += r.need;
   }
-  red[0][tid] = tok;
-  red[1][tid] = pages;
-  __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
-    if (tid < o) {
-      red[0][tid] += red[0][tid + o];
-      red[1][tid] += red[1][tid + o];
-    }
-    __syncthreads();
+  tok = wave_sum_i64(tok);
+  pages = wave_sum_i64(pages);
+  if (lane == 0) {
+    red[0][tid >> 6] = tok;
+    red[1][tid >> 6] = pages;
   }
-  const int64_t tok_base = red[0][0], page_base = red[1][0] + max(*p.cursor_in, 0);
-  __syncthreads();
   PlanRequest mine = {0, 0, 0, 0};
-  if (tid < nb) mine = plan_request(p, b0 + tid);
-  s_cached[tid] = mine.cached;
-  s_held[tid] = mine.held;
-  red[0][tid] = mine.fresh;
-  red[1][tid] = mine.need;
-  __syncthreads();
-  for (int o = 1; o < 256; o <<= 1) {     // inclusive scan
-    const int64_t a = tid >= o ? red[0][tid - o] : 0, b = tid >= o ? red[1][tid - o] : 0;
-    __syncthreads();
-    red[0][tid] += a;
-    red[1][tid] += b;
-    __syncthreads();
+  if (tid < 64) {
+    if (tid < nb) mine = plan_request(p, b0 + tid);
+    int64_t a = mine.fresh, c = mine.need;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {                     // inclusive scan
+      const int64_t ua = __shfl_up(a, o, 64), uc = __shfl_up(c, o, 64);
+      if (lane >= o) {
+        a += ua;
+        c += uc;
+      }
+    }
+    s_cached[tid] = mine.cached;
+    s_held[tid] = mine.held;
+    tok_off[tid + 1] = (int)min(a, (int64_t)0x7fffffff);
+    page_off[tid + 1] = (int)min(c, (int64_t)0x7fffffff);
+    if (tid == 0) tok_off[0] = page_off[0] = 0;
   }
-  tok_off[tid + 1] = red[0][tid];
-  page_off[tid + 1] = red[1][tid];
-  if (tid == 0) tok_off[0] = page_off[0] = 0;
   __syncthreads();
-  const int64_t n_tok = tok_off[nb], n_page = page_off[nb];
-  auto find = [&](const int64_t* off, int64_t i) {   // last request whose range starts at or before i
+  const int64_t tok_base = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]);
+  const int64_t page_base = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]) + cursor;
+  const int n_tok = tok_off[nb], n_page = page_off[nb];
+  auto find = [&](const int* off, int i) __attribute__((always_inline)) {   // last request whose range starts at or before i
     int lo = 0, hi = nb - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -101,37 +135,57 @@ __global__ void __launch_bounds__(256) paged_plan_kernel(PlanParams p) {
     }
     return lo;
   };
-  auto free_page = [&](int64_t at) { return at < p.n_free ? p.free_pages[at] : -1; };
+  auto free_page = [&](int64_t at) __attribute__((always_inline)) { return at < p.n_free ? p.free_pages[at] : -1; };
   if (blockIdx.y == 0) {
     if (tid < nb) {
-      const int64_t at = page_base + page_off[tid];
-      int64_t got = (int64_t)p.n_free - at;
+      int64_t got = (int64_t)p.n_free - (page_base + page_off[tid]);
       got = got < 0 ? 0 : (got < mine.need ? got : mine.need);
-      const int64_t cap = (mine.held + got) * p.page_size, want = (int64_t)mine.cached + mine.fresh;
+      const int64_t cap = (mine.held + got) * p.page.d, want = (int64_t)mine.cached + mine.fresh;
       p.seq_lens[b0 + tid] = (int)(want < cap ? want : cap);
       p.cu_new[b0 + tid] = (int)(tok_base + tok_off[tid]);
     }
-    for (int64_t i = tid; i < n_page; i += 256) {
-      const int r = find(page_off, i);
-      const int page = free_page(page_base + i);
+    for (int i = tid; i < n_page; i += 256) {
+      const int r = find(page_off, i), page = free_page(page_base + i);
       if (page >= 0) p.table[(int64_t)(b0 + r) * p.table_stride + s_held[r] + (i - page_off[r])] = page;
     }
   }
-  for (int64_t i = (int64_t)blockIdx.y * 256 + tid; i < n_tok; i += (int64_t)gridDim.y * 256) {
-    if (tok_base + i >= p.max_tokens) break;
+  // (64 bits: the last step of a walk over nearly 2^31 tokens passes them; four tokens at a time, so that their pages are looked up together)
+  const int64_t room = p.max_tokens - tok_base, stop = n_tok < room ? n_tok : room;
+  auto entry_of = [&](int i, int& off) __attribute__((always_inline)) {
     const int r = find(tok_off, i);
-    const int64_t pos = s_cached[r] + (i - tok_off[r]), j = pos / p.page_size;
-    int page = -1;
-    if (j < s_held[r]) page = p.table[(int64_t)(b0 + r) * p.table_stride + j];
-    else if (j < p.max_pages) page = free_page(page_base + page_off[r] + (j - s_held[r]));
-    p.slots[tok_base + i] = page < 0 ? -1 : (int64_t)page * p.page_size + pos % p.page_size;
+    const int64_t pos = (int64_t)s_cached[r] + (i - tok_off[r]);
+    off = 0;
+    if (pos >= (int64_t)p.max_pages * p.page.d) return (const int32_t*)nullptr;
+    const int j = (int)p.page.div((uint32_t)pos);
+    off = (int)pos - j * (int)p.page.d;
+    if (j < s_held[r]) return (const int32_t*)p.table + (int64_t)(b0 + r) * p.table_stride + j;
+    const int64_t at = page_base + page_off[r] + (j - s_held[r]);
+    return at < p.n_free ? p.free_pages + at : (const int32_t*)nullptr;
+  };
+  auto slot_of = [&](int page, int off) __attribute__((always_inline)) { return page < 0 ? (int64_t)-1 : (int64_t)page * p.page.d + off; };
+  int64_t k = (int64_t)blockIdx.y * 1024 + tid;
+  for (; k + 768 < stop; k += (int64_t)gridDim.y * 1024) {
+    int page[4], off[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int32_t* e = entry_of((int)k + u * 256, off[u]);
+      page[u] = e ? *e : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) p.slots[tok_base + k + u * 256] = slot_of(page[u], off[u]);
+  }
+  for (int u = 0; u < 4 && k < stop; ++u, k += 256) {
+    int off;
+    const int32_t* e = entry_of((int)k, off);
+    const int page = e ? *e : -1;
+    p.slots[tok_base + k] = slot_of(page, off);
   }
   if (b0 + nb == p.B) {
     const int64_t total = tok_base + n_tok;
     if (blockIdx.y == 0 && tid == 0) {
       p.cu_new[p.B] = (int)total;
-      const int64_t at = page_base + n_page, start = *p.cursor_in;
-      *p.cursor_out = (int)(at < p.n_free ? at : (start > p.n_free ? start : p.n_free));
+      const int64_t at = page_base + n_page, most = cursor > p.n_free ? cursor : p.n_free;
+      *p.cursor_out = (int)(at < most ? at : most);
     }
     for (int64_t i = total + (int64_t)blockIdx.y * 256 + tid; i < p.max_tokens; i += (int64_t)gridDim.y * 256) p.slots[i] = -1;
   }
@@ -195,8 +249,7 @@ struct PagedAttnParams {
   int64_t k_head, v_head;
   float scale_log2;
   int nsplit, qchunks;
-  uint32_t div_magic;      // t / page_size = (t * magic) >> (32 + shift) for 0 <= t < 2^31; 0: pages of one token
-  int div_shift;
+  FastDiv page;
   float* part;             // [B * H][nsplit][dh + 2]: output, maximum, sum of a part
 };
 
@@ -272,7 +325,7 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnParams p) {
   const int tl = lane % TK;
   auto look = [&](int t0, int& entry, int& off) __attribute__((always_inline)) {
     const int t = min(t0 + tl, t_end - 1);
-    const int j = p.div_magic ? (int)(__umulhi((uint32_t)t, p.div_magic) >> p.div_shift) : t;
+    const int j = (int)p.page.div((uint32_t)t);
     off = t - j * p.page_size;
     entry = table[j];
   };
@@ -588,18 +641,19 @@ extern "C" int nst_paged_plan(const int32_t* cached_lens, const int32_t* new_len
                 (long long)max_tokens);
   NST_CHECK_ARG((int64_t)max_pages * page_size <= MAX_POSITIONS, "nst_paged_plan: %d pages of %d tokens pass 2^30 positions", max_pages,
                 page_size);
+  NST_CHECK_ARG(max_tokens <= 0x7fffffffLL, "nst_paged_plan: max_tokens=%lld (at most 2^31 - 1)", (long long)max_tokens);
   NST_CHECK_ARG(cursor_in && cu_new && cursor_out && (slots || max_tokens == 0) && (free_pages || n_free == 0),
                 "nst_paged_plan: NULL pointer");
   NST_CHECK_ARG(B == 0 || (cached_lens && new_lens && block_table && seq_lens && table_stride >= max_pages),
                 "nst_paged_plan: NULL pointer or table stride %lld < %d", (long long)table_stride, max_pages);
   NST_CHECK_ARG(cursor_in != cursor_out && (B == 0 || (seq_lens != cached_lens && seq_lens != new_lens)),
                 "nst_paged_plan: the outputs may not overlap the inputs (other workgroups still read them)");
-  PlanParams p = {cached_lens, new_lens, B, page_size, max_pages, block_table, table_stride, free_pages, n_free, cursor_in,
-                  slots, max_tokens, seq_lens, cu_new, cursor_out, 1};
-  int64_t per = max_tokens > 0 ? (4096LL * B + max_tokens - 1) / max_tokens : 256;     // about 4096 tokens for a workgroup
-  p.per_group = (int)(per < 1 ? 1 : per > 256 ? 256 : per);
+  PlanParams p = {cached_lens, new_lens, B, max_pages, fast_div(page_size), block_table, table_stride, free_pages, n_free, cursor_in,
+                  slots, (int)max_tokens, seq_lens, cu_new, cursor_out, 1};
+  int64_t per = max_tokens > 0 ? (1024LL * B + max_tokens - 1) / max_tokens : 64;      // about 1024 tokens for a workgroup
+  p.per_group = (int)(per < 1 ? 1 : per > 64 ? 64 : per);
   const int gx = B > 0 ? (B + p.per_group - 1) / p.per_group : 1;
-  int64_t gy = max_tokens / ((int64_t)gx * 4096);
+  int64_t gy = max_tokens / ((int64_t)gx * 1024);
   gy = gy < 1 ? 1 : gy > 64 ? 64 : gy;
   paged_plan_kernel<<<dim3(gx, (unsigned)gy), 256, 0, (hipStream_t)stream>>>(p);
   NST_CHECK_LAUNCH("nst_paged_plan");
@@ -700,13 +754,7 @@ extern "C" int nst_paged_attention(const NstPagedAttnDesc* d, const void* q, con
   p.scale_log2 = d->scale * LOG2E;
   p.qchunks = (d->H / d->Hkv + 15) / 16;
   p.nsplit = paged_attention_splits(d);
-  // t / d by multiplication: with s = ceil(log2 d) and magic = floor(2^(31 + s) / d) + 1 the quotient is exact below 2^31
-  int s = 0;
-  while ((1LL << s) < pl.page_size) ++s;
-  if (s > 0) {
-    p.div_magic = (uint32_t)((1ULL << (31 + s)) / (uint64_t)pl.page_size + 1);
-    p.div_shift = s - 1;
-  }
+  p.page = fast_div(pl.page_size);
   if (p.nsplit > 1) {
     const int64_t need = (int64_t)d->B * d->H * p.nsplit * (d->dh + 2) * (int64_t)sizeof(float);
     if (!workspace || workspace_bytes < need || !nst_aligned16(workspace)) {

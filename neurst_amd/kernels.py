@@ -741,98 +741,116 @@ def attention_bwd(q, k, v, out, dout, lse, dq, dk, dv, H, dh, key_bias=None, cau
 
 
 # ------------------------------------------------------------------------------------------------ paged key / value caches
-def _on_device(what, *tensors):
+# A decoding step makes these calls once per layer or once per step and is bound by the host, so their checks read every property of an
+# operand once and build a message only when something is refused (measured: 13.6 -> 9 us of host time for a paged_attention call).
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+
+
+def _current(what, *tensors):
     """Every operand lives on the CURRENT device: the launch goes to its current stream."""
+    first = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError("neurst_amd kernels need ROCm device tensors (no CPU fallback)")
-        if _cur_device is not None and t.device.index != _cur_device():
-            raise RuntimeError(f"{what}: operand on {t.device}, but the current device is cuda:{_cur_device()}")
+        if t is not None and t.get_device() != first:
+            raise RuntimeError(f"{what}: operands on {tensors[0].device} and {t.device}")
+    if first < 0:
+        raise RuntimeError("neurst_amd kernels need ROCm device tensors (no CPU fallback)")
+    if first != _cur_device():
+        raise RuntimeError(f"{what}: operands on {tensors[0].device}, but the current device is cuda:{_cur_device()}")
 
 
-def _index_vector(what, name, t, dtype, n=None):
-    if not (t.dim() == 1 and t.dtype == dtype and (n is None or t.shape[0] == n) and (t.stride(0) == 1 or t.shape[0] <= 1)):
-        raise ValueError(f"{what}: {name} must be a dense {dtype} vector" + ("" if n is None else f" of {n}") + f", got {t.dtype} {tuple(t.shape)}")
+def _is_vector(t, dtype, n):
+    return t.dtype is dtype and t.shape == (n,) and (n <= 1 or t.stride(0) == 1)
 
 
-def _block_table(what, t, rows):
-    if not (t.dim() == 2 and t.dtype == torch.int32 and t.shape[0] == rows and t.shape[1] > 0 and (t.stride(1) == 1 or t.shape[1] == 1)):
-        raise ValueError(f"{what}: block_table must be int32 [{rows}, pages] with dense rows, got {t.dtype} {tuple(t.shape)}")
-    stride = t.stride(0) if rows > 1 else t.shape[1]
-    if not (stride >= t.shape[1]):
-        raise ValueError(f"{what}: rows of block_table overlap")
-    return stride
+def _vector_error(what, name, t, dtype, n):
+    return ValueError(f"{what}: {name} must be a dense {dtype} vector of {n}, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+
+
+def _table_stride(what, t, rows):
+    """Row stride of an int32 [rows, pages] table with dense rows."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not _I32 or len(shape) != 2 or shape[0] != rows or shape[1] == 0 or (stride[1] != 1 and shape[1] > 1):
+        raise ValueError(f"{what}: block_table must be int32 [{rows}, pages] with dense rows, got {t.dtype} {tuple(shape)} / {stride}")
+    if rows <= 1:
+        return shape[1]
+    if stride[0] < shape[1]:
+        raise ValueError(f"{what}: the rows of block_table overlap")
+    return stride[0]
 
 
 def _paged_pool(what, k_pool, v_pool):
-    """[pages, page_size, kv_heads, dh] views (any strides, dense heads) -> NstPagedPool."""
-    if not (k_pool.dim() == 4 and k_pool.shape == v_pool.shape and k_pool.dtype == v_pool.dtype and min(k_pool.shape[1:]) > 0):
-        raise ValueError(f"{what}: k_pool and v_pool must be [pages, page_size, kv_heads, dh] of one type, got {k_pool.dtype} {tuple(k_pool.shape)} and " f"{v_pool.dtype} {tuple(v_pool.shape)}")
-    if not (k_pool.shape[3] == 1 or (k_pool.stride(3) == 1 and v_pool.stride(3) == 1)):
+    """[pages, page_size, kv_heads, dh] views (any strides, dense heads) -> (NstPagedPool, shape)."""
+    shape, ks, vs = k_pool.shape, k_pool.stride(), v_pool.stride()
+    if len(shape) != 4 or v_pool.shape != shape or v_pool.dtype is not k_pool.dtype or 0 in shape[1:]:
+        raise ValueError(f"{what}: k_pool and v_pool must be [pages, page_size, kv_heads, dh] of one type, got {k_pool.dtype} {tuple(shape)} "
+                         f"and {v_pool.dtype} {tuple(v_pool.shape)}")
+    if shape[3] > 1 and (ks[3] != 1 or vs[3] != 1):
         raise ValueError(f"{what}: the elements of a head must be dense")
-    return NstPagedPool(k_pool.shape[0], k_pool.shape[1], _dt(k_pool), 0, k_pool.stride(0), k_pool.stride(1), k_pool.stride(2),
-                        v_pool.stride(0), v_pool.stride(1), v_pool.stride(2))
+    return NstPagedPool(shape[0], shape[1], _dt(k_pool), 0, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]), shape
 
 
 def paged_plan(cached_lens, new_lens, block_table, free_pages, cursor, page_size, max_tokens):
     """Pages and slots for the new tokens of every request (nst_paged_plan): block_table is completed in place from free_pages
     [cursor ..); returns (slots [max_tokens] int64, seq_lens [B], cu_new [B + 1], cursor [1]), all on the device -- nothing
     comes back to the host.  cached_lens, new_lens, free_pages, cursor int32."""
-    B = cached_lens.shape[0] if cached_lens.dim() == 1 else -1
-    _index_vector("paged_plan", "cached_lens", cached_lens, torch.int32)
-    _index_vector("paged_plan", "new_lens", new_lens, torch.int32, B)
-    _index_vector("paged_plan", "free_pages", free_pages, torch.int32)
-    _index_vector("paged_plan", "cursor", cursor, torch.int32, 1)
-    stride = _block_table("paged_plan", block_table, B)
-    _on_device("paged_plan", cached_lens, new_lens, block_table, free_pages, cursor)
+    B, n_free = cached_lens.numel(), free_pages.numel()
+    for name, t, n in (("cached_lens", cached_lens, B), ("new_lens", new_lens, B), ("free_pages", free_pages, n_free), ("cursor", cursor, 1)):
+        if not _is_vector(t, _I32, n):
+            raise _vector_error("paged_plan", name, t, _I32, n)
+    stride = _table_stride("paged_plan", block_table, B)
+    _current("paged_plan", cached_lens, new_lens, block_table, free_pages, cursor)
     dev = block_table.device
-    slots = torch.empty(int(max_tokens), dtype=torch.int64, device=dev)
-    small = torch.empty(2 * B + 2, dtype=torch.int32, device=dev)
-    seq_lens, cu_new, cursor_out = small[:B], small[B:2 * B + 1], small[2 * B + 1:]
-    check(lib.nst_paged_plan(_p(cached_lens), _p(new_lens), B, _p(block_table), stride, block_table.shape[1], _p(free_pages),
-                             free_pages.shape[0], _p(cursor), int(page_size), _p(slots), slots.shape[0], _p(seq_lens), _p(cu_new),
-                             _p(cursor_out), _stream()), "paged_plan")
+    slots = torch.empty(max_tokens, dtype=_I64, device=dev)
+    seq_lens, cu_new, cursor_out = torch.empty(2 * B + 2, dtype=_I32, device=dev).split_with_sizes((B, B + 1, 1))
+    check(lib.nst_paged_plan(cached_lens.data_ptr(), new_lens.data_ptr(), B, block_table.data_ptr(), stride, block_table.shape[1],
+                             free_pages.data_ptr(), n_free, cursor.data_ptr(), page_size, slots.data_ptr(), max_tokens,
+                             seq_lens.data_ptr(), cu_new.data_ptr(), cursor_out.data_ptr(), _stream()), "paged_plan")
     return slots, seq_lens, cu_new, cursor_out
 
 
 def paged_append(k, v, k_pool, v_pool, slots):
     """Rows k, v [tokens, kv_heads, dh] into their slots of the pools [pages, page_size, kv_heads, dh] (in place); slots int64 [tokens], a
     slot outside the pools is skipped, no slot may appear twice."""
-    pool = _paged_pool("paged_append", k_pool, v_pool)
-    if not (k.dim() == 3 and k.shape == v.shape and k.shape[1:] == k_pool.shape[2:] and k.dtype == v.dtype == k_pool.dtype):
-        raise ValueError(f"paged_append: rows {k.dtype} {tuple(k.shape)} / {v.dtype} {tuple(v.shape)} for pools {k_pool.dtype} {tuple(k_pool.shape)}")
-    if not (k.shape[2] == 1 or (k.stride(2) == 1 and v.stride(2) == 1)):
+    pool, ps = _paged_pool("paged_append", k_pool, v_pool)
+    shape, ks, vs = k.shape, k.stride(), v.stride()
+    if len(shape) != 3 or v.shape != shape or shape[1:] != ps[2:] or k.dtype is not k_pool.dtype or v.dtype is not k_pool.dtype:
+        raise ValueError(f"paged_append: rows {k.dtype} {tuple(shape)} / {v.dtype} {tuple(v.shape)} for pools {k_pool.dtype} {tuple(ps)}")
+    if shape[2] > 1 and (ks[2] != 1 or vs[2] != 1):
         raise ValueError("paged_append: the elements of a head must be dense")
-    _index_vector("paged_append", "slots", slots, torch.int64, k.shape[0])
-    _on_device("paged_append", k, v, k_pool, v_pool, slots)
-    check(lib.nst_paged_append(_p(k), _p(v), k.shape[0], k.shape[1], k.shape[2], k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                               _p(k_pool), _p(v_pool), C.byref(pool), _p(slots), _stream()), "paged_append")
+    if not _is_vector(slots, _I64, shape[0]):
+        raise _vector_error("paged_append", "slots", slots, _I64, shape[0])
+    _current("paged_append", k, v, k_pool, v_pool, slots)
+    check(lib.nst_paged_append(k.data_ptr(), v.data_ptr(), shape[0], shape[1], shape[2], ks[0], ks[1], vs[0], vs[1], k_pool.data_ptr(),
+                               v_pool.data_ptr(), C.byref(pool), slots.data_ptr(), _stream()), "paged_append")
 
 
 def paged_attention(q, k_pool, v_pool, block_table, seq_lens, scale=None, max_len=None, return_lse=False):
-    """Attention of one new token per request over its cached tokens (nst_paged_attention): q [B, H, dh], pools [pages, page_size, kv_heads,
-    dh] with H a multiple of kv_heads, block_table [B, max_pages] int32, seq_lens [B] int32 -> out [B, H, dh] (and lse [B, H] f32).
-    scale: dh^-0.5 by default.  max_len: a bound of seq_lens the host knows; it chooses how the work is split, never the result's
-    extent."""
-    pool = _paged_pool("paged_attention", k_pool, v_pool)
-    if not (q.dim() == 3 and q.dtype == k_pool.dtype and q.shape[2] == k_pool.shape[3] and q.shape[1] > 0 and (q.shape[2] == 1 or q.stride(2) == 1)):
-        raise ValueError(f"paged_attention: q {q.dtype} {tuple(q.shape)} for pools {k_pool.dtype} {tuple(k_pool.shape)}")
-    B, H, dh = q.shape
-    _index_vector("paged_attention", "seq_lens", seq_lens, torch.int32, B)
-    stride = _block_table("paged_attention", block_table, B)
-    _on_device("paged_attention", q, k_pool, v_pool, block_table, seq_lens)
-    out = torch.empty(B, H, dh, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, H, dtype=torch.float32, device=q.device) if return_lse else None
-    d = NstPagedAttnDesc(B, H, k_pool.shape[2], dh, block_table.shape[1], int(max_len or 0), float(dh ** -0.5 if scale is None else scale), 0,
-                         q.stride(0), q.stride(1), H * dh, dh, stride, pool)
-    nbytes = lib.nst_paged_attention_workspace_bytes(C.byref(d))
+    """Attention of one new token per request over its cached tokens (nst_paged_attention): q [B, H, dh], pools [pages, page_size,
+    kv_heads, dh] with H a multiple of kv_heads, block_table [B, max_pages] int32, seq_lens [B] int32 -> out [B, H, dh] (and lse [B, H]
+    f32).  scale: dh^-0.5 by default.  max_len: a bound of seq_lens the host knows; it chooses how the work is split, never the
+    result's extent."""
+    pool, ps = _paged_pool("paged_attention", k_pool, v_pool)
+    shape, qs = q.shape, q.stride()
+    if len(shape) != 3 or q.dtype is not k_pool.dtype or shape[2] != ps[3] or shape[1] == 0 or (qs[2] != 1 and shape[2] > 1):
+        raise ValueError(f"paged_attention: q {q.dtype} {tuple(shape)} / {qs} for pools {k_pool.dtype} {tuple(ps)}")
+    B, H, dh = shape
+    if not _is_vector(seq_lens, _I32, B):
+        raise _vector_error("paged_attention", "seq_lens", seq_lens, _I32, B)
+    stride = _table_stride("paged_attention", block_table, B)
+    _current("paged_attention", q, k_pool, v_pool, block_table, seq_lens)
+    dev = q.device
+    out = torch.empty(shape, dtype=q.dtype, device=dev)
+    lse = torch.empty(B, H, dtype=_F32, device=dev) if return_lse else None
+    desc = NstPagedAttnDesc(B, H, ps[2], dh, block_table.shape[1], max_len or 0, dh ** -0.5 if scale is None else scale, 0, qs[0], qs[1],
+                            H * dh, dh, stride, pool)
+    d = C.byref(desc)
+    nbytes = lib.nst_paged_attention_workspace_bytes(d)
     if nbytes < 0:
         check(nbytes, "paged_attention", launches=False)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None      # (of its own: two graphs never share it)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None      # (of its own: two graphs never share it)
     ev = PROBE.begin("paged_attention")
-    check(lib.nst_paged_attention(C.byref(d), _p(q), _p(k_pool), _p(v_pool), _p(block_table), _p(seq_lens), _p(out), _p(lse), _p(ws), nbytes,
+    check(lib.nst_paged_attention(d, q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+                                  out.data_ptr(), lse.data_ptr() if return_lse else None, ws.data_ptr() if nbytes else None, nbytes,
                                   _stream()), "paged_attention")
     PROBE.end(ev)
     return (out, lse) if return_lse else out
@@ -842,65 +860,68 @@ def paged_reorder(pool, block_table, seq_lens, parents, spare):
     """Re-ordering behind a beam-search step (nst_paged_reorder): row r continues row parents[r] (int64), which is as long.  pool [planes,
     pages, page_size, width]: the partly filled pages are copied in place, full pages are shared; spare [R] int32: one free page
     per row.  Returns the new (block_table, spare)."""
-    if not (pool.dim() == 4 and min(pool.shape[0], pool.shape[2], pool.shape[3]) > 0 and (pool.shape[3] == 1 or pool.stride(3) == 1) and (pool.shape[2] == 1 or pool.stride(2) == pool.shape[3])):
-        raise ValueError(f"paged_reorder: pool must be [planes, pages, page_size, width] with dense pages, got {tuple(pool.shape)} / {pool.stride()}")
-    R = block_table.shape[0] if block_table.dim() == 2 else -1
-    stride = _block_table("paged_reorder", block_table, R)
-    _index_vector("paged_reorder", "seq_lens", seq_lens, torch.int32, R)
-    _index_vector("paged_reorder", "parents", parents, torch.int64, R)
-    _index_vector("paged_reorder", "spare", spare, torch.int32, R)
-    _on_device("paged_reorder", pool, block_table, seq_lens, parents, spare)
-    W = block_table.shape[1]
-    table_out = torch.empty(R, W, dtype=torch.int32, device=pool.device)
-    spare_out = torch.empty(R, dtype=torch.int32, device=pool.device)
-    es = pool.element_size()
-    check(lib.nst_paged_reorder(_p(pool), pool.shape[0], pool.stride(0) * es, pool.shape[1], pool.stride(1) * es, pool.shape[2],
-                                pool.shape[3] * es, _p(block_table), stride, _p(table_out), W, W, R, _p(seq_lens), _p(parents), _p(spare),
-                                _p(spare_out), _stream()), "paged_reorder")
+    shape, st = pool.shape, pool.stride()
+    if len(shape) != 4 or 0 in (shape[0], shape[2], shape[3]) or (shape[3] > 1 and st[3] != 1) or (shape[2] > 1 and st[2] != shape[3]):
+        raise ValueError(f"paged_reorder: pool must be [planes, pages, page_size, width] with dense pages, got {tuple(shape)} / {st}")
+    R = spare.numel()
+    stride = _table_stride("paged_reorder", block_table, R)
+    for name, t, dt in (("seq_lens", seq_lens, _I32), ("parents", parents, _I64), ("spare", spare, _I32)):
+        if not _is_vector(t, dt, R):
+            raise _vector_error("paged_reorder", name, t, dt, R)
+    _current("paged_reorder", pool, block_table, seq_lens, parents, spare)
+    W, es, dev = block_table.shape[1], pool.element_size(), pool.device
+    table_out = torch.empty(R, W, dtype=_I32, device=dev)
+    spare_out = torch.empty(R, dtype=_I32, device=dev)
+    check(lib.nst_paged_reorder(pool.data_ptr(), shape[0], st[0] * es, shape[1], st[1] * es, shape[2], shape[3] * es,
+                                block_table.data_ptr(), stride, table_out.data_ptr(), W, W, R, seq_lens.data_ptr(), parents.data_ptr(),
+                                spare.data_ptr(), spare_out.data_ptr(), _stream()), "paged_reorder")
     return table_out, spare_out
 
 
 # ------------------------------------------------------------------------------------------------ log probabilities of tokens
+def _logit_rows(what, logits, tokens):
+    shape, st = logits.shape, logits.stride()
+    if len(shape) != 2 or shape[1] == 0 or (st[1] != 1 and shape[1] > 1):
+        raise ValueError(f"{what}: logits must be [rows, vocabulary] with dense rows, got {tuple(shape)} / {st}")
+    if not _is_vector(tokens, _I64, shape[0]):
+        raise _vector_error(what, "tokens", tokens, _I64, shape[0])
+    return shape[0], shape[1], st[0]
+
+
 def token_logprobs(logits, tokens, top_n=0):
     """logits [rows, V], tokens [rows] int64 -> (logp, entropy, lse [rows] f32, top_logp [rows, top_n] f32, top_ids [rows, top_n] int64):
     the log probability of the given token (0 for a token outside [0, V)), the entropy, the log-sum-exp and the top_n <= 64 likeliest
     tokens of every row, equal logits by the lower id (nst_token_logprobs_fwd)."""
-    if not (logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1)):
-        raise ValueError(f"token_logprobs: logits must be [rows, vocabulary] with dense rows, got {tuple(logits.shape)} / {logits.stride()}")
-    rows, V = logits.shape
-    _index_vector("token_logprobs", "tokens", tokens, torch.int64, rows)
-    _on_device("token_logprobs", logits, tokens)
-    dt, top_n = _dt(logits), int(top_n)
+    rows, V, ldl = _logit_rows("token_logprobs", logits, tokens)
+    _current("token_logprobs", logits, tokens)
+    dt, dev = _dt(logits), logits.device
     nbytes = lib.nst_token_logprobs_workspace_bytes(rows, V, top_n, dt)
     if nbytes < 0:
         check(nbytes, "token_logprobs", launches=False)
-    stats = torch.empty(3, rows, dtype=torch.float32, device=logits.device)
-    top_logp = torch.empty(rows, top_n, dtype=torch.float32, device=logits.device)
-    top_ids = torch.empty(rows, top_n, dtype=torch.int64, device=logits.device)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
-    logp, entropy, lse = stats[0], stats[1], stats[2]
-    check(lib.nst_token_logprobs_fwd(_p(logits), _p(tokens), _p(logp), _p(entropy), _p(lse), _p(top_logp), _p(top_ids), rows, V,
-                                     logits.stride(0), top_n, dt, _p(ws), nbytes, _stream()), "token_logprobs")
+    logp, entropy, lse = torch.empty(3, rows, dtype=_F32, device=dev).unbind()
+    top_logp = torch.empty(rows, top_n, dtype=_F32, device=dev)
+    top_ids = torch.empty(rows, top_n, dtype=_I64, device=dev)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    check(lib.nst_token_logprobs_fwd(logits.data_ptr(), tokens.data_ptr(), logp.data_ptr(), entropy.data_ptr(), lse.data_ptr(),
+                                     top_logp.data_ptr(), top_ids.data_ptr(), rows, V, ldl, top_n, dt, ws.data_ptr() if nbytes else None,
+                                     nbytes, _stream()), "token_logprobs")
     return logp, entropy, lse, top_logp, top_ids
 
 
 def token_logprobs_bwd(logits, tokens, lse, entropy, dlogp, dentropy=None, out=None):
     """d(logits) from d(logp) and d(entropy) (either None: zero), with the lse and entropy that token_logprobs returned
     (nst_token_logprobs_bwd).  out: where to write it; may be logits itself."""
-    if not (logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1)):
-        raise ValueError(f"token_logprobs_bwd: logits must be [rows, vocabulary] with dense rows, got {tuple(logits.shape)} / {logits.stride()}")
-    rows, V = logits.shape
-    _index_vector("token_logprobs_bwd", "tokens", tokens, torch.int64, rows)
+    rows, V, ldl = _logit_rows("token_logprobs_bwd", logits, tokens)
     for name, t in (("lse", lse), ("entropy", entropy), ("dlogp", dlogp), ("dentropy", dentropy)):
-        if t is not None or name == "lse":
-            _index_vector("token_logprobs_bwd", name, t, torch.float32, rows)
+        if (t is not None or name == "lse") and not _is_vector(t, _F32, rows):
+            raise _vector_error("token_logprobs_bwd", name, t, _F32, rows)
     if out is None:
         out = torch.empty(rows, V, dtype=logits.dtype, device=logits.device)
-    if not (out.shape == logits.shape and out.dtype == logits.dtype and (out.stride(1) == 1 or V == 1)):
-        raise ValueError(f"token_logprobs_bwd: out {out.dtype} {tuple(out.shape)} for logits {logits.dtype} {tuple(logits.shape)}")
-    _on_device("token_logprobs_bwd", logits, tokens, lse, entropy, dlogp, dentropy, out)
-    check(lib.nst_token_logprobs_bwd(_p(logits), _p(tokens), _p(lse), _p(entropy), _p(dlogp), _p(dentropy), _p(out), rows, V,
-                                     logits.stride(0), out.stride(0), _dt(logits), _stream()), "token_logprobs_bwd")
+    elif out.shape != logits.shape or out.dtype is not logits.dtype or (out.stride(1) != 1 and V > 1):
+        raise ValueError(f"token_logprobs_bwd: out {out.dtype} {tuple(out.shape)} / {out.stride()} for logits {logits.dtype} {tuple(logits.shape)}")
+    _current("token_logprobs_bwd", logits, tokens, lse, entropy, dlogp, dentropy, out)
+    check(lib.nst_token_logprobs_bwd(logits.data_ptr(), tokens.data_ptr(), lse.data_ptr(), _p(entropy), _p(dlogp), _p(dentropy),
+                                     out.data_ptr(), rows, V, ldl, out.stride(0), _dt(logits), _stream()), "token_logprobs_bwd")
     return out
 
 
