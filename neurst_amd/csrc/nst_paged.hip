@@ -12,6 +12,7 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
+constexpr float LOWEST = -3.402823466e38f;
 constexpr int64_t MAX_POSITIONS = 1 << 30;     // of one request: position arithmetic, a tile or two past the end included, stays in 32 bits
 
 // t / d for 0 <= t < 2^31 by one multiplication: with s = ceil(log2 d) and magic = floor(2^(31 + s) / d) + 1 the error of t * magic / 2^(31 + s)
@@ -250,7 +251,8 @@ struct PagedAttnParams {
   float scale_log2;
   int nsplit, qchunks;
   FastDiv page;
-  float* part;             // [B * H][nsplit][dh + 2]: output, maximum, sum of a part
+  float* part_ml;          // [B * H][nsplit][2]: maximum and sum of a part
+  float* part_o;           // [B * H][nsplit][dh rounded up to 4]: its output
 };
 
 template <typename T>
@@ -317,7 +319,7 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnParams p) {
   floatx4_t acc[NA];
 #pragma unroll
   for (int i = 0; i < NA; ++i) acc[i] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-  float m = -3.402823466e38f, l = 0.f;
+  float m = LOWEST, l = 0.f;
   uint4 kr[NF][KC], vr[BF ? VC : NF * 4 * (DP / 64 > 0 ? DP / 64 : 1)];
 
   // Lane i looks up the page of token t0 + i % TK.  The entry is checked where it is used, a tile later: a check here would wait for it,
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnParams p) {
     valid = __ballot(ok);
     return ok ? entry : 0;
   };
-  auto load = [&](int page, int off) __attribute__((always_inline)) {
+  auto load_k = [&](int page, int off) __attribute__((always_inline)) {
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       const uint32_t pg = __shfl(page, f * 16 + lc, 64), of = __shfl(off, f * 16 + lc, 64);
@@ -343,6 +345,8 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnParams p) {
 #pragma unroll
       for (int c = 0; c < KC; ++c) kr[f][c] = row_chunk<T, VEC>(row, c * (64 / (int)sizeof(T)) + g * PA<T>::E, dh);
     }
+  };
+  auto load_v = [&](int page, int off) __attribute__((always_inline)) {
     if constexpr (BF) {
 #pragma unroll
       for (int i = 0; i < VC; ++i) {
@@ -374,7 +378,8 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnParams p) {
     const int page = resolve(t0, entry, next_valid);
     const int o = off;
     look(t0 + 4 * TK, entry, off);
-    load(page, o);
+    load_k(page, o);
+    load_v(page, o);
   }
   for (; t0 < t_end; t0 += 4 * TK) {
     const uint64_t valid = next_valid;
@@ -409,23 +414,19 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnParams p) {
         }
       }
     }
-    floatx4_t vcur[BF ? 1 : NF * 4 * (DP / 64 > 0 ? DP / 64 : 1)];
     if constexpr (BF) {
 #pragma unroll
       for (int i = 0; i < VC; ++i) {
         const int r = (i * 64 + lane) / (DP / 8), col = (i * 64 + lane) % (DP / 8);
         *reinterpret_cast<uint4*>(vt + r * RSV + col * 16) = vr[i];
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NF * 4 * (DP / 64); ++i) vcur[i] = __builtin_bit_cast(floatx4_t, vr[i]);
     }
-    // ---- the next tile's rows on their way, and the pages of the one behind it (past the end: rows and entries that exist, unused)
-    {
-      const int page = resolve(t0 + 4 * TK, entry, next_valid), o = off;
-      look(t0 + 8 * TK, entry, off);
-      load(page, o);
-    }
+    // ---- the next tile's rows on their way, and the pages of the one behind it (past the end: rows and entries that exist, unused).
+    // f32 keeps V in its load registers until the second product: a copy would cost half of the waves a SIMD can hold
+    const int next_page = resolve(t0 + 4 * TK, entry, next_valid), next_off = off;
+    look(t0 + 8 * TK, entry, off);
+    load_k(next_page, next_off);
+    if constexpr (BF) load_v(next_page, next_off);
     // ---- weights
     float mx = -INFINITY;
 #pragma unroll
@@ -477,7 +478,9 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnParams p) {
           for (int c = 0; c < DP / 64; ++c)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              acc[c * 4 + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vcur[(f * 4 + r) * (DP / 64) + c][j], s[f][r], acc[c * 4 + j], 0, 0, 0);
+              acc[c * 4 + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(floatx4_t, vr[(f * 4 + r) * (DP / 64) + c])[j], s[f][r],
+                                                                    acc[c * 4 + j], 0, 0, 0);
+      load_v(next_page, next_off);
     }
   }
   l += __shfl_xor(l, 16, 64);
@@ -513,12 +516,9 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnParams p) {
     }
     const int64_t row = (int64_t)b * p.H + h0 + h;
     if (p.nsplit > 1) {
-      float* dst = p.part + (row * p.nsplit + split) * (p.dh + 2);
-      dst[d] = o;
-      if (d == 0) {
-        dst[p.dh] = mj;
-        dst[p.dh + 1] = lj;
-      }
+      const int64_t at = row * p.nsplit + split;
+      p.part_o[at * ((dh + 3) & ~3) + d] = o;
+      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mj, lj);
     } else {
       ((T*)p.out)[b * p.o_row + (h0 + h) * p.o_head + d] = from_f32<T>(lj == 0.f ? 0.f : o / lj);
       if (d == 0 && p.lse) p.lse[row] = lj == 0.f ? -INFINITY : (mj + log2f(lj)) * LN2;
@@ -526,36 +526,64 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnParams p) {
   }
 }
 
-// Joins the parts of a request: one workgroup per (request, head); wave w takes parts w, w + 4, ..., a lane the dims lane + 64 i.
+// Joins the parts of a request: one workgroup per (request, head).  The weights of all parts first (they need every maximum), then threads
+// of four dims each share the parts, eight reads of each in flight: with 256 parts this is all the time there is.
+constexpr int MAX_SPLITS = 2048;
 template <typename T>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(PagedAttnParams p) {
-  __shared__ float s_o[4][256], s_m[4], s_l[4];
+  __shared__ float s_w[MAX_SPLITS], s_red[2][4];
+  __shared__ float4 s_o[256];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t row = blockIdx.x;
   const int b = (int)(row / p.H), h = (int)(row - (int64_t)b * p.H);
-  const int len = min(max(p.lens[b], 0), p.max_pages * p.page_size);
+  const int len = min(max(p.lens[b], 0), p.max_pages * (int)p.page.d);
   const int part = part_tokens(len, p.nsplit), n = (int)(((int64_t)len + part - 1) / part);
-  const float* src = p.part + row * p.nsplit * (p.dh + 2);
-  float m = -3.402823466e38f;
-  for (int i = lane; i < n; i += 64) m = fmaxf(m, src[(int64_t)i * (p.dh + 2) + p.dh]);
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row * p.nsplit;
+  float m = LOWEST;
+  for (int i = tid; i < n; i += 256) m = fmaxf(m, ml[i].x);
   m = wave_max(m);
-  float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = wave; i < n; i += 4) {
-    const float* s = src + (int64_t)i * (p.dh + 2);
-    const float c = __builtin_amdgcn_exp2f(s[p.dh] - m);
-    l += c * s[p.dh + 1];
+  if (lane == 0) s_red[0][wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+  float l = 0.f;
+  for (int i = tid; i < n; i += 256) {
+    const float2 v = ml[i];
+    const float w = __builtin_amdgcn_exp2f(v.x - m);
+    s_w[i] = w;
+    l += w * v.y;
+  }
+  l = wave_sum(l);
+  if (lane == 0) s_red[1][wave] = l;
+  __syncthreads();
+  l = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+  const int dv = (p.dh + 3) / 4;                           // threads of one part (<= 64); `groups` parts at a time
+  const int groups = 256 / dv, grp = tid / dv, c = tid - grp * dv;
+  const float4* src = reinterpret_cast<const float4*>(p.part_o) + row * p.nsplit * dv + c;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (grp < groups) {
+    for (int i = grp; i < n; i += groups * 8) {
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = src[(int64_t)min(i + k * groups, n - 1) * dv];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = i + k * groups < n ? s_w[i + k * groups] : 0.f;
+        o.x += w * v[k].x; o.y += w * v[k].y; o.z += w * v[k].z; o.w += w * v[k].w;
+      }
+    }
+  }
+  s_o[tid] = o;
+  __syncthreads();
+  if (tid < dv) {
+    for (int k = 1; k < groups; ++k) {
+      const float4 v = s_o[k * dv + tid];
+      o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+    }
+    const float r[4] = {o.x, o.y, o.z, o.w};
+    T* dst = (T*)p.out + b * p.o_row + h * p.o_head + tid * 4;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (k * 64 + lane < p.dh) o[k] += c * s[k * 64 + lane];
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) s_o[wave][k * 64 + lane] = o[k];
-  if (lane == 0) s_l[wave] = l;
-  __syncthreads();
-  l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
-  if (tid < p.dh) {
-    const float v = (s_o[0][tid] + s_o[1][tid]) + (s_o[2][tid] + s_o[3][tid]);
-    ((T*)p.out)[b * p.o_row + h * p.o_head + tid] = from_f32<T>(l == 0.f ? 0.f : v / l);
+      if (tid * 4 + k < p.dh) dst[k] = from_f32<T>(l == 0.f ? 0.f : r[k] / l);
   }
   if (tid == 0 && p.lse) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
 }
@@ -713,20 +741,28 @@ static int paged_attention_check(const NstPagedAttnDesc* d) {
   return NST_OK;
 }
 
-// How many parts a request is cut into at most.  Enough workgroups for every CU to hold several, but no part below MIN_PART tokens.
+// How many parts a request is cut into at most: 1024 workgroups (four for a CU), and parts of at most 2048 tokens, or the last long requests
+// of a ragged batch run alone (64 requests of 1 .. 8192 tokens: 240 us with 1024 workgroups alone, 226 us so; parts half as long
+// 230 us), but none below MIN_PART.
 static int paged_attention_splits(const NstPagedAttnDesc* d) {
   const int64_t cap = (int64_t)d->max_pages * d->pool.page_size, bound = d->max_len > 0 && d->max_len < cap ? d->max_len : cap;
   const int64_t units = (int64_t)d->B * d->Hkv * ((d->H / d->Hkv + 15) / 16);
-  const int64_t most = (bound + MIN_PART - 1) / MIN_PART, want = (2048 + units - 1) / units;
-  const int64_t n = want < most ? want : most;
-  return (int)(n < 1 ? 1 : n);
+  const int64_t most = (bound + MIN_PART - 1) / MIN_PART, few = (1024 + units - 1) / units, ragged = (bound + 2047) / 2048;
+  const int64_t want = few > ragged ? few : ragged, n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n > MAX_SPLITS ? MAX_SPLITS : n);
+}
+
+static int64_t paged_attention_ml_bytes(const NstPagedAttnDesc* d, int nsplit) {      // (the outputs behind it start 16-byte aligned)
+  return ((int64_t)d->B * d->H * nsplit * 8 + 15) / 16 * 16;
+}
+static int64_t paged_attention_workspace(const NstPagedAttnDesc* d, int nsplit) {
+  return nsplit > 1 ? paged_attention_ml_bytes(d, nsplit) + (int64_t)d->B * d->H * nsplit * ((d->dh + 3) / 4 * 16) : 0;
 }
 
 extern "C" int64_t nst_paged_attention_workspace_bytes(const NstPagedAttnDesc* d) {
   const int rc = paged_attention_check(d);
   if (rc != NST_OK) return rc;
-  const int n = d->B > 0 ? paged_attention_splits(d) : 1;
-  return n > 1 ? (int64_t)d->B * d->H * n * (d->dh + 2) * (int64_t)sizeof(float) : 0;
+  return d->B > 0 ? paged_attention_workspace(d, paged_attention_splits(d)) : 0;
 }
 
 extern "C" int nst_paged_attention(const NstPagedAttnDesc* d, const void* q, const void* k_pool, const void* v_pool,
@@ -756,12 +792,13 @@ extern "C" int nst_paged_attention(const NstPagedAttnDesc* d, const void* q, con
   p.nsplit = paged_attention_splits(d);
   p.page = fast_div(pl.page_size);
   if (p.nsplit > 1) {
-    const int64_t need = (int64_t)d->B * d->H * p.nsplit * (d->dh + 2) * (int64_t)sizeof(float);
+    const int64_t need = paged_attention_workspace(d, p.nsplit);
     if (!workspace || workspace_bytes < need || !nst_aligned16(workspace)) {
       nst_set_error("nst_paged_attention: workspace of %lld bytes, needs %lld (16-byte aligned)", (long long)workspace_bytes, (long long)need);
       return NST_ERR_WORKSPACE;
     }
-    p.part = (float*)workspace;
+    p.part_ml = (float*)workspace;
+    p.part_o = (float*)((char*)workspace + paged_attention_ml_bytes(d, p.nsplit));
   }
   const int64_t blocks = (int64_t)d->B * d->Hkv * p.qchunks * p.nsplit;
   NST_CHECK_ARG(blocks <= 0x7fffffffLL, "nst_paged_attention: %lld workgroups", (long long)blocks);
