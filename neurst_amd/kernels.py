@@ -744,18 +744,21 @@ def attention_bwd(q, k, v, out, dout, lse, dq, dk, dv, H, dh, key_bias=None, cau
 # A decoding step makes these calls once per layer or once per step and is bound by the host, so their checks read every property of an
 # operand once and build a message only when something is refused (measured: 13.6 -> 9 us of host time for a paged_attention call).
 _I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
+_DT = {torch.float32: NST_F32, torch.bfloat16: NST_BF16}
 
 
-def _current(what, *tensors):
-    """Every operand lives on the CURRENT device: the launch goes to its current stream."""
-    first = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != first:
-            raise RuntimeError(f"{what}: operands on {tensors[0].device} and {t.device}")
-    if first < 0:
-        raise RuntimeError("neurst_amd kernels need ROCm device tensors (no CPU fallback)")
-    if first != _cur_device():
-        raise RuntimeError(f"{what}: operands on {tensors[0].device}, but the current device is cuda:{_cur_device()}")
+def _device_error(what, *tensors):
+    """Some operand is not on the CURRENT device, whose current stream the launch goes to."""
+    if any(t is not None and not t.is_cuda for t in tensors):
+        return RuntimeError("neurst_amd kernels need ROCm device tensors (no CPU fallback)")
+    return RuntimeError(f"{what}: operands on {sorted({str(t.device) for t in tensors if t is not None})}, but the current device is "
+                        f"cuda:{torch.cuda.current_device()}")
+
+
+def _here(t):
+    """The device of t if that is the current one, else -2, which is no tensor's."""
+    dev = t.get_device()
+    return dev if dev >= 0 and dev == _cur_device() else -2
 
 
 def _is_vector(t, dtype, n):
@@ -779,14 +782,17 @@ def _table_stride(what, t, rows):
 
 
 def _paged_pool(what, k_pool, v_pool):
-    """[pages, page_size, kv_heads, dh] views (any strides, dense heads) -> (NstPagedPool, shape)."""
+    """[pages, page_size, kv_heads, dh] views (any strides, dense heads) -> (the fields of NstPagedPool, shape)."""
     shape, ks, vs = k_pool.shape, k_pool.stride(), v_pool.stride()
     if len(shape) != 4 or v_pool.shape != shape or v_pool.dtype is not k_pool.dtype or 0 in shape[1:]:
         raise ValueError(f"{what}: k_pool and v_pool must be [pages, page_size, kv_heads, dh] of one type, got {k_pool.dtype} {tuple(shape)} "
                          f"and {v_pool.dtype} {tuple(v_pool.shape)}")
     if shape[3] > 1 and (ks[3] != 1 or vs[3] != 1):
         raise ValueError(f"{what}: the elements of a head must be dense")
-    return NstPagedPool(shape[0], shape[1], _dt(k_pool), 0, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]), shape
+    dt = _DT.get(k_pool.dtype)
+    if dt is None:
+        raise TypeError(f"unsupported dtype {k_pool.dtype}")
+    return (shape[0], shape[1], dt, 0, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]), shape
 
 
 def paged_plan(cached_lens, new_lens, block_table, free_pages, cursor, page_size, max_tokens):
@@ -798,7 +804,9 @@ def paged_plan(cached_lens, new_lens, block_table, free_pages, cursor, page_size
         if not _is_vector(t, _I32, n):
             raise _vector_error("paged_plan", name, t, _I32, n)
     stride = _table_stride("paged_plan", block_table, B)
-    _current("paged_plan", cached_lens, new_lens, block_table, free_pages, cursor)
+    if not (_here(block_table) == cached_lens.get_device() == new_lens.get_device() == block_table.get_device() == free_pages.get_device()
+            == cursor.get_device()):
+        raise _device_error("paged_plan", cached_lens, new_lens, block_table, free_pages, cursor)
     dev = block_table.device
     slots = torch.empty(max_tokens, dtype=_I64, device=dev)
     seq_lens, cu_new, cursor_out = torch.empty(2 * B + 2, dtype=_I32, device=dev).split_with_sizes((B, B + 1, 1))
@@ -819,9 +827,10 @@ def paged_append(k, v, k_pool, v_pool, slots):
         raise ValueError("paged_append: the elements of a head must be dense")
     if not _is_vector(slots, _I64, shape[0]):
         raise _vector_error("paged_append", "slots", slots, _I64, shape[0])
-    _current("paged_append", k, v, k_pool, v_pool, slots)
+    if not (_here(k_pool) == v_pool.get_device() == k.get_device() == v.get_device() == slots.get_device()):
+        raise _device_error("paged_append", k, v, k_pool, v_pool, slots)
     check(lib.nst_paged_append(k.data_ptr(), v.data_ptr(), shape[0], shape[1], shape[2], ks[0], ks[1], vs[0], vs[1], k_pool.data_ptr(),
-                               v_pool.data_ptr(), C.byref(pool), slots.data_ptr(), _stream()), "paged_append")
+                               v_pool.data_ptr(), C.byref(NstPagedPool(*pool)), slots.data_ptr(), _stream()), "paged_append")
 
 
 def paged_attention(q, k_pool, v_pool, block_table, seq_lens, scale=None, max_len=None, return_lse=False):
@@ -837,12 +846,13 @@ def paged_attention(q, k_pool, v_pool, block_table, seq_lens, scale=None, max_le
     if not _is_vector(seq_lens, _I32, B):
         raise _vector_error("paged_attention", "seq_lens", seq_lens, _I32, B)
     stride = _table_stride("paged_attention", block_table, B)
-    _current("paged_attention", q, k_pool, v_pool, block_table, seq_lens)
+    if not (_here(q) == k_pool.get_device() == v_pool.get_device() == block_table.get_device() == seq_lens.get_device()):
+        raise _device_error("paged_attention", q, k_pool, v_pool, block_table, seq_lens)
     dev = q.device
     out = torch.empty(shape, dtype=q.dtype, device=dev)
     lse = torch.empty(B, H, dtype=_F32, device=dev) if return_lse else None
     desc = NstPagedAttnDesc(B, H, ps[2], dh, block_table.shape[1], max_len or 0, dh ** -0.5 if scale is None else scale, 0, qs[0], qs[1],
-                            H * dh, dh, stride, pool)
+                            H * dh, dh, stride, pool)      # (a tuple fills the nested structure)
     d = C.byref(desc)
     nbytes = lib.nst_paged_attention_workspace_bytes(d)
     if nbytes < 0:
@@ -868,7 +878,8 @@ def paged_reorder(pool, block_table, seq_lens, parents, spare):
     for name, t, dt in (("seq_lens", seq_lens, _I32), ("parents", parents, _I64), ("spare", spare, _I32)):
         if not _is_vector(t, dt, R):
             raise _vector_error("paged_reorder", name, t, dt, R)
-    _current("paged_reorder", pool, block_table, seq_lens, parents, spare)
+    if not (_here(pool) == block_table.get_device() == seq_lens.get_device() == parents.get_device() == spare.get_device()):
+        raise _device_error("paged_reorder", pool, block_table, seq_lens, parents, spare)
     W, es, dev = block_table.shape[1], pool.element_size(), pool.device
     table_out = torch.empty(R, W, dtype=_I32, device=dev)
     spare_out = torch.empty(R, dtype=_I32, device=dev)
@@ -893,7 +904,8 @@ def token_logprobs(logits, tokens, top_n=0):
     the log probability of the given token (0 for a token outside [0, V)), the entropy, the log-sum-exp and the top_n <= 64 likeliest
     tokens of every row, equal logits by the lower id (nst_token_logprobs_fwd)."""
     rows, V, ldl = _logit_rows("token_logprobs", logits, tokens)
-    _current("token_logprobs", logits, tokens)
+    if _here(logits) != tokens.get_device():
+        raise _device_error("token_logprobs", logits, tokens)
     dt, dev = _dt(logits), logits.device
     nbytes = lib.nst_token_logprobs_workspace_bytes(rows, V, top_n, dt)
     if nbytes < 0:
@@ -919,7 +931,10 @@ def token_logprobs_bwd(logits, tokens, lse, entropy, dlogp, dentropy=None, out=N
         out = torch.empty(rows, V, dtype=logits.dtype, device=logits.device)
     elif out.shape != logits.shape or out.dtype is not logits.dtype or (out.stride(1) != 1 and V > 1):
         raise ValueError(f"token_logprobs_bwd: out {out.dtype} {tuple(out.shape)} / {out.stride()} for logits {logits.dtype} {tuple(logits.shape)}")
-    _current("token_logprobs_bwd", logits, tokens, lse, entropy, dlogp, dentropy, out)
+    dev = _here(logits)
+    for t in (tokens, lse, entropy, dlogp, dentropy, out):
+        if t is not None and t.get_device() != dev:
+            raise _device_error("token_logprobs_bwd", logits, tokens, lse, entropy, dlogp, dentropy, out)
     check(lib.nst_token_logprobs_bwd(logits.data_ptr(), tokens.data_ptr(), lse.data_ptr(), _p(entropy), _p(dlogp), _p(dentropy),
                                      out.data_ptr(), rows, V, ldl, out.stride(0), _dt(logits), _stream()), "token_logprobs_bwd")
     return out
