@@ -146,7 +146,7 @@ class MultiHeadSelfAttention(MultiHeadAttention):
     def forward(self, x, B, T, bias=None, causal=False, is_training=True, epilogue=None, cache=None):
         """x [B*T, d]; bias [B,T] f32 key-padding bias or None; causal=True is the decoder's lower-triangle bias.
         cache (inference only): {"keys", "values": [B, Tmax, d] buffers, "len": filled positions}; T == 1 for a decoding
-        step, T >= 1 for a chunk of the streaming encoder."""
+        step, T >= 1 for a chunk of the streaming encoder.  Or {"paged": PagedKVCache, "layer": its layer, "len"} for decoding steps."""
         d, H, dh = self.num_units, self.num_heads, self.dh
         p = self.rate if is_training else 0.0
         qkv = self.qkv_transform.forward(x)
@@ -156,6 +156,14 @@ class MultiHeadSelfAttention(MultiHeadAttention):
             # (transformer_encoder.py:138-175 builds lower_triangle_attention_bias(t + T)[:, :, -T:]).
             assert not is_training
             t = cache["len"]
+            if "paged" in cache:
+                if T != 1:
+                    raise NotImplementedError("a paged cache takes one position per row and step")
+                rows = qkv.view(B, 3, H, dh)
+                cache["paged"].append(cache["layer"], rows[:, 1], rows[:, 2])
+                cache["len"] = t + 1
+                ctx = cache["paged"].attend(cache["layer"], rows[:, 0])
+                return self.output_transform.forward(ctx.view(B, d), **(epilogue or {}))
             if t + T > cache["keys"].shape[1]:
                 raise RuntimeError(f"attention cache of {cache['keys'].shape[1]} positions is full")
             v3 = qkv.view(B, T, 3 * d)

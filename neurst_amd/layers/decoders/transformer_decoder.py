@@ -5,6 +5,7 @@ import torch
 
 from neurst_amd import kernels as K
 from neurst_amd.layers import layer_utils
+from neurst_amd.layers.attentions.paged_kv_cache import PagedKVCache
 from neurst_amd.layers.common_layers import LayerNorm, ResidualStream, dropped_grad
 from neurst_amd.layers.decoders.decoder import Decoder, register_decoder
 from neurst_amd.layers.transformer_layers import TransformerDecoderLayer
@@ -66,10 +67,12 @@ class TransformerDecoder(Decoder):
         return kv_all
 
     def create_decoding_internal_cache(self, encoder_outputs, encoder_inputs_padding, is_inference=False,
-                                       decode_padded_length=None):
+                                       decode_padded_length=None, page_size=None, static=False):
         """transformer_decoder.py:105-147.  Training: {"decoding_states": None, "memory", "memory_bias"}.  Inference adds
         per-layer decoding states: self-attention key / value buffers of `decode_padded_length` positions (filled one
-        position per step) and the cross attention's projected memory (filled at the first step)."""
+        position per step) and the cross attention's projected memory (filled at the first step).
+        page_size: keep the self-attention keys and values in pages of that many positions instead (PagedKVCache; static: for
+        captured graphs)."""
         cache = dict(decoding_states=None)
         if encoder_inputs_padding is not None:
             cache["memory"] = encoder_outputs
@@ -78,6 +81,13 @@ class TransformerDecoder(Decoder):
             if decode_padded_length is None:
                 raise ValueError("inference needs decode_padded_length (the maximum number of decoding steps)")
             B, d = encoder_outputs.shape[0], self._params["hidden_size"]
+            if page_size:
+                H, L = self._params["num_attention_heads"], self._params["num_layers"]
+                paged = PagedKVCache(L, B, H, d // H, decode_padded_length, page_size, encoder_outputs.dtype, encoder_outputs.device, static)
+                cache["decoding_states"] = {f"layer_{i}": {"self_attention": {"paged": paged, "layer": i, "len": 0}, "encdec_attention": {}}
+                                            for i in range(L)}
+                cache["paged"] = paged
+                return cache
             # one buffer for the keys and values of all layers: a beam re-ordering is ONE gather over it
             kv_all = torch.zeros(self._params["num_layers"], 2, B, decode_padded_length, d, dtype=encoder_outputs.dtype,
                                  device=encoder_outputs.device)
@@ -127,6 +137,9 @@ class TransformerDecoder(Decoder):
         """tf.gather(cache, beam_ids) of the beam search (beam_search.py:409-410): only the self-attention buffers depend on
         the hypothesis; memory, memory_bias and the projected memory are identical for all beams of a sample (beam_ids
         never leave the sample's block), so they stay in place."""
+        if "paged" in cache:
+            cache["paged"].reorder(beam_ids)
+            return cache
         n = next(iter(cache["decoding_states"].values()))["self_attention"]["len"]
         kv = cache["self_attention_kv"]
         kv[:, :, :, :n] = kv[:, :, :, :n].index_select(2, beam_ids)
@@ -146,6 +159,8 @@ class TransformerDecoder(Decoder):
             memory_bias = torch.minimum(memory_bias, layer_utils.FLOAT_MIN * (1.0 - seen)[None, :])
         if memory_bias is not None and not memory_bias.is_contiguous():
             memory_bias = memory_bias.contiguous()           # the kernel reads a dense [B, Tk] bias
+        if "paged" in cache:
+            cache["paged"].extend()
         x = decoder_inputs
         if self._stream32:
             x = ResidualStream(x if x.is_contiguous() else x.contiguous())

@@ -14,6 +14,7 @@ HIP path).  Semantics kept from the reference:
 """
 import torch
 
+from neurst_amd import kernels as K
 from neurst_amd.utils.flags_core import Flag
 from neurst_amd.utils.registry import setup_registry
 
@@ -50,14 +51,41 @@ def length_penalty_term(lengths, alpha, dtype=torch.float32):
     return ((5.0 + lengths) / 6.0) ** (-alpha)
 
 
+def _fused_next_word(logits, log_probs, lengths, finished, beam_base, batch, beam_size, banned, eos_id, length_penalty, time):
+    """One expansion over the n = beam + |banned| likeliest symbols of every hypothesis: at most |banned| of them may not be taken, so the
+    beam_size best of a hypothesis -- and with them the beam_size best of the sample -- are among them.  A finished hypothesis offers EOS at
+    no cost and nothing else."""
+    n = beam_size + len(banned)
+    l2 = logits.reshape(-1, logits.shape[-1])
+    top_lp, top_ids = K.token_logprobs(l2, torch.zeros(l2.shape[0], dtype=torch.int64, device=l2.device), n)[3:]
+    for b in banned:
+        top_lp = torch.where(top_ids == b, top_lp + FLOAT_MIN, top_lp)
+    fin = finished[:, None]
+    only_eos = torch.full((n,), FLOAT_MIN, dtype=torch.float32, device=l2.device)
+    only_eos[0] = 0.0
+    top_lp = torch.where(fin, only_eos[None, :], top_lp)
+    top_ids = torch.where(fin, torch.full_like(top_ids, eos_id), top_ids)
+    total = top_lp + log_probs[:, None]
+    next_len = lengths + 1 - finished.long()
+    scores = (total * length_penalty_term(next_len, length_penalty)[:, None]).view(batch, beam_size * n)
+    if time == 0:
+        scores = scores[:, :n]
+    sample = torch.topk(scores, k=beam_size, dim=-1)[1].reshape(-1)
+    beam_ids = torch.div(sample, n, rounding_mode="floor") + beam_base
+    at = beam_base * n + sample
+    return top_ids.reshape(-1).index_select(0, at), beam_ids, total.reshape(-1).index_select(0, at), next_len
+
+
 def sequence_beam_search(symbols_to_logits_fn, generation_initializer, top_k=1, beam_size=4, length_penalty=0.6,
                          extra_decode_length=50, maximum_decode_length=256, minimum_decode_length=0, enable_unk=False,
-                         reorder_cache_fn=None, ensemble_weights=None):
+                         reorder_cache_fn=None, ensemble_weights=None, fused_scores=False):
     """generation_initializer: {"decoder_input": int tensor [batch], "decoder_internal_cache": cache ALREADY stacked to
     batch * beam rows by the caller (the model owns its layout), "encoder_inputs_maxlen": int | None, "eos_id", "unk_id"}.
     symbols_to_logits_fn(ids [batch*beam], cache, time) -> logits [batch*beam, vocab], or a list of them (an ENSEMBLE:
     the step distribution is sum_i ensemble_weights[i] * softmax(logits_i), beam_search.py:104-116).
-    reorder_cache_fn(cache, beam_ids) -> cache re-ordered like tf.gather(cache, beam_ids)."""
+    reorder_cache_fn(cache, beam_ids) -> cache re-ordered like tf.gather(cache, beam_ids).
+    fused_scores: only the likeliest symbols of a hypothesis are ranked, found with their log probabilities in one kernel over the logits
+    (kernels.token_logprobs) instead of a log-softmax and a top-k over the vocabulary.  The same hypotheses, up to ties; not for ensembles."""
     ids = generation_initializer["decoder_input"]
     cache = generation_initializer["decoder_internal_cache"]
     enc_len = generation_initializer.get("encoder_inputs_maxlen", None)
@@ -78,6 +106,18 @@ def sequence_beam_search(symbols_to_logits_fn, generation_initializer, top_k=1, 
     # EOS at zero cost (log-prob, length and ranking unchanged), the returned hypotheses are the same
     while time < max_steps and not (time % 4 == 0 and time > 0 and bool(finished.all())):
         logits = symbols_to_logits_fn(input_ids, cache, time)
+        banned = ([] if unk_id is None else [unk_id]) + ([eos_id] if time < minimum_decode_length - 1 else [])
+        if fused_scores and torch.is_tensor(logits) and beam_size + len(banned) <= min(64, logits.shape[-1]):
+            word_ids, beam_ids, log_probs, next_len = _fused_next_word(logits, log_probs, lengths, finished, beam_base, batch, beam_size, banned,
+                                                                       eos_id, length_penalty, time)
+            lengths = next_len.index_select(0, beam_ids)
+            predicted = torch.cat([predicted.index_select(0, beam_ids), word_ids[:, None]], dim=1)
+            if reorder_cache_fn is not None:
+                cache = reorder_cache_fn(cache, beam_ids)
+            finished = word_ids == eos_id
+            input_ids = word_ids
+            time += 1
+            continue
         if isinstance(logits, (list, tuple)) and len(logits) > 1:
             w = torch.as_tensor(ensemble_weights, dtype=torch.float32, device=dev)
             assert w.numel() == len(logits), "one ensemble weight per sub-model"
@@ -128,14 +168,14 @@ class BeamSearch(SequenceSearch):
     """SequenceSearch "beam_search" (beam_search.py:443-551): binds the search hyper-parameters, drives a model."""
 
     def __init__(self, args=None, beam_size=4, length_penalty=0.6, top_k=1, maximum_decode_length=None, minimum_decode_length=0,
-                 extra_decode_length=50, enable_unk=False, use_graphs=False):
+                 extra_decode_length=50, enable_unk=False, use_graphs=False, page_size=None, fused_scores=False):
         a = dict(beam_size=beam_size, length_penalty=length_penalty, top_k=top_k, maximum_decode_length=maximum_decode_length,
                  minimum_decode_length=minimum_decode_length, extra_decode_length=extra_decode_length, enable_unk=enable_unk,
-                 use_graphs=use_graphs)
+                 use_graphs=use_graphs, page_size=page_size, fused_scores=fused_scores)
         a.update({k: v for k, v in (args or {}).items() if v is not None and k in a})
         if (args or {}).get("padded_decode", None):
             pass  # the cache is preallocated to the maximum length anyway: nothing to switch
-        self.use_graphs = bool(a["use_graphs"])
+        self.use_graphs, self.page_size, self.fused_scores = bool(a["use_graphs"]), a["page_size"] or None, bool(a["fused_scores"])
         self.beam_size, self.length_penalty, self.top_k = a["beam_size"], a["length_penalty"], a["top_k"]
         self.maximum_decode_length, self.minimum_decode_length = a["maximum_decode_length"], a["minimum_decode_length"] or 0
         self.extra_decode_length, self.enable_unk = a["extra_decode_length"], bool(a["enable_unk"])
@@ -154,6 +194,10 @@ class BeamSearch(SequenceSearch):
             Flag("padded_decode", dtype=Flag.TYPE.BOOLEAN, default=None, help="Accepted for compatibility (static cache always)."),
             Flag("enable_unk", dtype=Flag.TYPE.BOOLEAN, default=None, help="Whether the search may generate UNK."),
             Flag("use_graphs", dtype=Flag.TYPE.BOOLEAN, default=None, help="Replay the decoding step as a captured HIP graph."),
+            Flag("page_size", dtype=Flag.TYPE.INTEGER, default=None,
+                 help="Keep the decoder's self-attention keys and values in pages of that many positions (default: a dense cache)."),
+            Flag("fused_scores", dtype=Flag.TYPE.BOOLEAN, default=None,
+                 help="Rank only the likeliest symbols of a hypothesis, found in one kernel over the logits."),
         ]
 
     def __call__(self, model, inputs, ensemble_weights=None):
@@ -163,11 +207,12 @@ class BeamSearch(SequenceSearch):
         kw = dict(top_k=self.top_k, beam_size=self.beam_size, length_penalty=self.length_penalty,
                   extra_decode_length=self.extra_decode_length, maximum_decode_length=max_len,
                   minimum_decode_length=self.minimum_decode_length, enable_unk=self.enable_unk)
+        paged = {"page_size": self.page_size} if self.page_size else {}
         if not isinstance(model, (list, tuple)):
             fn, init, reorder = model.get_symbols_to_logits_fn(inputs, beam_size=self.beam_size, decode_padded_length=max_len,
-                                                               use_graphs=self.use_graphs)
-            return sequence_beam_search(fn, init, reorder_cache_fn=reorder, **kw)
-        parts = [m.get_symbols_to_logits_fn(inputs, beam_size=self.beam_size, decode_padded_length=max_len) for m in model]
+                                                               use_graphs=self.use_graphs, **paged)
+            return sequence_beam_search(fn, init, reorder_cache_fn=reorder, fused_scores=self.fused_scores, **kw)
+        parts = [m.get_symbols_to_logits_fn(inputs, beam_size=self.beam_size, decode_padded_length=max_len, **paged) for m in model]
         if ensemble_weights is None or ensemble_weights == "average":
             ensemble_weights = [1.0 / len(parts)] * len(parts)
         init = dict(parts[0][1], decoder_internal_cache=[p[1]["decoder_internal_cache"] for p in parts])

@@ -24,20 +24,25 @@ class _DecodeSession(object):
     lengths; step(ids, cache, t) replays graph t (capturing it the first time: an eager warm-up run, then the capture of
     the same step -- writing position t twice is idempotent)."""
 
-    def __init__(self, decoder, eager_step, memory, padding, max_len):
+    def __init__(self, decoder, eager_step, memory, padding, max_len, page_size=None):
         self.decoder, self.eager_step, self.max_len = decoder, eager_step, max_len
         self.memory, self.padding = memory.clone(), padding.clone()
-        self.cache = decoder.create_decoding_internal_cache(self.memory, self.padding, is_inference=True, decode_padded_length=max_len)
+        self.cache = decoder.create_decoding_internal_cache(self.memory, self.padding, is_inference=True, decode_padded_length=max_len,
+                                                            **({"page_size": page_size, "static": True} if page_size else {}))
         self.graphs, self.pool = {}, None
 
     def _set_len(self, n):
         for st in self.cache["decoding_states"].values():
             st["self_attention"]["len"] = n
+        if "paged" in self.cache:      # (the lengths the kernels read live on the device: a replay has brought them forward itself)
+            self.cache["paged"].len = n
 
     def begin(self, memory, padding):
         from neurst_amd.layers import layer_utils
         self.memory.copy_(memory)
         self.cache["memory_bias"].copy_(layer_utils.input_padding_to_bias(padding))
+        if "paged" in self.cache:
+            self.cache["paged"].reset()
         self._set_len(0)
         return self.cache, self.step
 
@@ -48,6 +53,8 @@ class _DecodeSession(object):
             static_ids = ids.clone()
             self._set_len(time)
             self.eager_step(static_ids, cache, time)          # warm-up: allocations, lazy state (projected memory at t = 0)
+            if "paged" in cache:
+                cache["paged"].rewind(time)
             self._set_len(time)
             if time == 0:  # the projection of the memory belongs INSIDE graph 0: every new batch must recompute it
                 for st in cache["decoding_states"].values():
@@ -219,14 +226,17 @@ class EncoderDecoderModel(BaseModel):
     __call__ = forward
 
     # ------------------------------------------------------------------ inference
-    def get_symbols_to_logits_fn(self, inputs, beam_size=1, decode_padded_length=256, use_graphs=False):
+    def get_symbols_to_logits_fn(self, inputs, beam_size=1, decode_padded_length=256, use_graphs=False, page_size=None):
         """encoder_decoder_model.py:187-260 for inference: runs the encoder once, builds the decoder's incremental cache for
         batch * beam rows and returns (symbols_to_logits_fn, generation_initializer, reorder_cache_fn) for
         neurst_amd.layers.search.sequence_beam_search.
 
         use_graphs: a decoding step is ~100 small launches and host-launch bound; with use_graphs the step of every time
         index is captured ONCE into a HIP graph over static buffers (ids in, logits out, the K/V caches and the encoder
-        memory in place) and replayed for every later batch of the same shape (see _DecodeSession)."""
+        memory in place) and replayed for every later batch of the same shape (see _DecodeSession).
+
+        page_size: the decoder's self-attention cache in pages of that many positions (layers/attentions/paged_kv_cache.py): a beam
+        re-ordering then copies less than a page per hypothesis instead of gathering every position of every layer."""
         from neurst_amd.layers.search.beam_search import stack_beam_size
         embedded_inputs = self._src_modality.forward(inputs["src"], is_training=False)
         src_padding = self._src_padding(inputs, embedded_inputs)
@@ -240,14 +250,14 @@ class EncoderDecoderModel(BaseModel):
             return self.output_logits_layer(hidden, is_training=False)
 
         if use_graphs:
-            key = (tuple(memory.shape), memory.dtype, decode_padded_length)
+            key = (tuple(memory.shape), memory.dtype, decode_padded_length) + ((page_size,) if page_size else ())
             sessions = self.__dict__.setdefault("_decode_sessions", {})
             if key not in sessions:
-                sessions[key] = _DecodeSession(self._decoder, eager_step, memory, padding, decode_padded_length)
+                sessions[key] = _DecodeSession(self._decoder, eager_step, memory, padding, decode_padded_length, page_size)
             cache, step_fn = sessions[key].begin(memory, padding)
         else:
-            cache = self._decoder.create_decoding_internal_cache(memory, padding, is_inference=True,
-                                                                 decode_padded_length=decode_padded_length)
+            cache = self._decoder.create_decoding_internal_cache(memory, padding, is_inference=True, decode_padded_length=decode_padded_length,
+                                                                 **({"page_size": page_size} if page_size else {}))
             step_fn = eager_step
         batch = encoder_outputs.shape[0]
         first = inputs.get("trg_input", None)

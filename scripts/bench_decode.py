@@ -24,6 +24,8 @@ def main():
     ap.add_argument("--max-len", type=int, default=75)
     ap.add_argument("--reps", type=int, default=3)
     ap.add_argument("--graphs", action="store_true", help="replay one captured HIP graph per decoding step")
+    ap.add_argument("--page-size", type=int, default=0, help="self-attention cache in pages of that many positions (0: dense)")
+    ap.add_argument("--fused-scores", action="store_true", help="rank only the likeliest symbols, found in one kernel over the logits")
     a = ap.parse_args()
     from neurst_amd.layers.search import BeamSearch
     from neurst_amd.models import build_model
@@ -36,7 +38,8 @@ def main():
     inputs = {"src": torch.randn(a.batch, a.frames, 80, 1, generator=g).to(dev),
               "src_length": torch.full((a.batch,), a.frames, dtype=torch.int64, device=dev)}
     search = BeamSearch(beam_size=a.beam, length_penalty=0.6, maximum_decode_length=a.max_len, extra_decode_length=0,
-                        minimum_decode_length=a.max_len, use_graphs=a.graphs)   # EOS masked until the last step: fixed amount of work
+                        minimum_decode_length=a.max_len, use_graphs=a.graphs, page_size=a.page_size or None,
+                        fused_scores=a.fused_scores)   # EOS masked until the last step: fixed amount of work
     hyp, _ = search(model, inputs)                          # warm-up
     torch.cuda.synchronize()
     t0 = time.time()
@@ -47,12 +50,14 @@ def main():
     # encoder alone
     t0 = time.time()
     for _ in range(a.reps):
-        model.get_symbols_to_logits_fn(inputs, beam_size=a.beam, decode_padded_length=a.max_len, use_graphs=a.graphs)
+        model.get_symbols_to_logits_fn(inputs, beam_size=a.beam, decode_padded_length=a.max_len, use_graphs=a.graphs,
+                                       **({"page_size": a.page_size} if a.page_size else {}))
     torch.cuda.synchronize()
     enc = (time.time() - t0) / a.reps
     steps = int(hyp.shape[1])
     out = {"metric": "beam-search decoding, SpeechTransformer (synthetic, random weights)", "model": a.model, "dtype": a.dtype,
            "batch": a.batch, "frames": a.frames, "beam_size": a.beam, "decode_steps": steps, "hip_graphs": bool(a.graphs),
+           "page_size": a.page_size, "fused_scores": bool(a.fused_scores),
            "ms_per_batch": total * 1e3, "ms_encoder_and_cache": enc * 1e3, "ms_per_decode_step": (total - enc) / steps * 1e3,
            "utterances_per_s": a.batch / total, "generated_tokens_per_s": a.batch * steps / total,
            "beam_tokens_per_s": a.batch * a.beam * steps / total}
