@@ -297,8 +297,9 @@ __global__ void __launch_bounds__(256) token_logprobs_kernel(LogprobParams p) {
   }
 }
 
-// Joins the parts of a row: lane i of every wave has part i (four waves only so that the lists arrive at once).  Alternatives: only the top_n parts with the largest heads can hold any, and of
-// those only what is not below the smallest of these heads.
+// Joins the parts of a row: lane i of every wave has part i (four waves only so that the lists arrive at once).  Alternatives: with d entries
+// of each list looked at (d * parts >= top_n), k = ceil(top_n / d) lists hold at least k * d >= top_n keys not below the k-th largest of the
+// lists' d-th entries, so only keys from it on are candidates; they are ranked by counting.
 template <typename T>
 __global__ void __launch_bounds__(256) token_logprobs_join_kernel(LogprobParams p) {
   extern __shared__ uint64_t lists[];                  // [nparts][top_n], then the lists' heads and, in their place, the candidates
@@ -312,9 +313,10 @@ __global__ void __launch_bounds__(256) token_logprobs_join_kernel(LogprobParams 
     m = q.x; s = q.y; t = q.z;
   }
   uint64_t *heads = lists + np * n, *cand = heads;
+  const int depth = n > 0 ? (n + np - 1) / np : 1, wanted = n > 0 ? (n + depth - 1) / depth : 0;      // d and k
   {
     const uint64_t* src = p.keys + row * np * n;
-    const uint64_t head = n > 0 && lane < np ? src[lane * n] : 0;
+    const uint64_t head = n > 0 && lane < np ? src[lane * n + depth - 1] : 0;
     uint64_t v[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = i * 256 + tid < np * n ? src[i * 256 + tid] : 0;
@@ -335,13 +337,13 @@ __global__ void __launch_bounds__(256) token_logprobs_join_kernel(LogprobParams 
   int rank = 0;
 #pragma unroll 8
   for (int j = 0; j < np; ++j) rank += heads[j] > head;
-  // (heads differ: a key holds its index, and no part is empty)
-  const uint64_t nth = __ballot(lane < np && rank == n - 1);
+  // (keys differ, a key holds its index; lists that are shorter than d have 0 there: then there may be no k-th, and every key counts)
+  const uint64_t nth = __ballot(lane < np && head != 0 && rank == wanted - 1);
   const uint64_t tau = nth ? heads[__ffsll((unsigned long long)nth) - 1] : 1;
   __syncthreads();                                      // the candidates take the heads' place
   if (tid < 64) {
     int cnt = 0;
-    if (lane < np && head >= tau)
+    if (lane < np)
       while (cnt < n && lists[lane * n + cnt] >= tau) ++cnt;
     int incl = cnt;
 #pragma unroll

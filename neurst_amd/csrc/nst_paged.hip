@@ -141,7 +141,8 @@ __global__ void __launch_bounds__(256) paged_plan_kernel(PlanParams p) {
     if (tid < nb) {
       int64_t got = (int64_t)p.n_free - (page_base + page_off[tid]);
       got = got < 0 ? 0 : (got < mine.need ? got : mine.need);
-      const int64_t cap = (mine.held + got) * p.page.d, want = (int64_t)mine.cached + mine.fresh;
+      const int64_t room = max((int64_t)p.max_tokens - (tok_base + tok_off[tid]), (int64_t)0);       // slots left for its tokens
+      const int64_t cap = (mine.held + got) * p.page.d, want = mine.cached + (mine.fresh < room ? mine.fresh : room);
       p.seq_lens[b0 + tid] = (int)(want < cap ? want : cap);
       p.cu_new[b0 + tid] = (int)(tok_base + tok_off[tid]);
     }

@@ -849,7 +849,7 @@ def paged_attention(q, k_pool, v_pool, block_table, seq_lens, scale=None, max_le
     if not (_here(q) == k_pool.get_device() == v_pool.get_device() == block_table.get_device() == seq_lens.get_device()):
         raise _device_error("paged_attention", q, k_pool, v_pool, block_table, seq_lens)
     dev = q.device
-    out = torch.empty(shape, dtype=q.dtype, device=dev)
+    out = torch.empty(B, H, dh, dtype=q.dtype, device=dev)
     lse = torch.empty(B, H, dtype=_F32, device=dev) if return_lse else None
     desc = NstPagedAttnDesc(B, H, ps[2], dh, block_table.shape[1], max_len or 0, dh ** -0.5 if scale is None else scale, 0, qs[0], qs[1],
                             H * dh, dh, stride, pool)      # (a tuple fills the nested structure)

@@ -613,7 +613,7 @@ def paged_plan(cached_lens, new_lens, block_table, free_pages, cursor, page_size
         got = min(max(n_free - at, 0), need)
         block_table[b, held:held + got] = free_pages[at:at + got]
         at += need
-        seq.append(min(cached + new, (held + got) * page_size))
+        seq.append(min(cached + min(new, max(int(max_tokens) - t, 0)), (held + got) * page_size))
         for pos in range(cached, cached + new):
             if t < max_tokens and pos // page_size < held + got:
                 page = int(block_table[b, pos // page_size])

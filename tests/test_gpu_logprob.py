@@ -95,6 +95,15 @@ def test_forward_over_sizes(K, rows, V, dtype):
             assert_forward(K, x, tokens, top_n)
 
 
+@pytest.mark.parametrize("kind", ["plain", "ties", "equal", "sorted", "few"])
+@pytest.mark.parametrize("rows,V", [(1, 2048), (1, 2049), (1, 5000), (3, 20000), (2, 45000), (100, 3000), (1, 1 << 20)])
+def test_alternatives_joined_from_parts(K, rows, V, kind):
+    """Rows cut into 2 .. 64 parts, fewer and more than the alternatives that are asked for."""
+    x = make_logits(rows, V, torch.float32, kind, seed=V)
+    for top_n in (1, 3, 10, 31, 50, 64):
+        assert_forward(K, x, torch.zeros(rows, dtype=torch.int64), top_n)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("kind", ["ties", "equal", "few", "inf", "sorted", "peaked", "signed zero"])
 @pytest.mark.parametrize("V", [70, 3001, 40000])

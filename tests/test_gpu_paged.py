@@ -251,7 +251,7 @@ def test_plan_matches_its_contract(K, B, cached_hi, new_hi, ps):
         at += int(held[b])
     free, cursor = pages[at:].contiguous(), i32([4])
     total = int(new.sum())
-    for extra in (0, 13):
+    for extra in (0, 13, -(total // 3)):          # (the last: fewer slots than tokens)
         t_ref = table.clone()
         t_dev = torch.full((B, W + 3), -1, dtype=torch.int32, device=DEV)[:, 1:W + 1]
         t_dev.copy_(table)
