@@ -410,14 +410,16 @@ __global__ void __launch_bounds__(256) token_logprobs_bwd_kernel(const T* logits
 struct LogprobSplit {
   int nparts, part, pieces;     // pieces: of a thread
 };
-// Rows of up to 16384 elements stay whole: cutting 16 rows of 8008 bf16 in 8 parts measured 5.6 us of device time without alternatives and
-// 9.5 us with six, whole rows 3.6 and 7.4 us (and a launch less for the host).  Longer ones are cut, into at most 64 parts of at most
-// 16384 elements -- and of at least 1024 where there are so few rows that they would not reach every CU otherwise.
+// Rows of up to 32768 elements stay whole.  Against parts of 1024 .. 16384 elements and a second launch (device time without / with six
+// alternatives): 16 rows of 8008 bf16 3.6 / 6.2 against 5.6 / 9.5 us, 127 rows of 32000 5.7 / 9.9 against 7.3 / 12.3 us, 1000 rows of
+// 32000 14.5 / 19.1 against 16.8 / 23.5 us, and a launch less for the host.  Longer ones are cut into at most 64 parts of at most 16384
+// elements (1000 rows of 50000 float32 34 us, in parts of up to 32768 35 us) -- of at least 1024 where there are so few rows that they
+// would not reach every CU otherwise.
 static LogprobSplit logprob_split(int64_t rows, int V, int dtype) {
   const int E = dtype == NST_BF16 ? 8 : 4, most = 16384;
-  int64_t want = V <= most || rows >= 128 ? 1 : rows > 0 ? (256 + rows - 1) / rows : 1;
+  int64_t want = V <= 2 * most || rows >= 128 ? 1 : rows > 0 ? (256 + rows - 1) / rows : 1;
   if (want > (V + 1023) / 1024) want = (V + 1023) / 1024;
-  if (want < (V + most - 1) / most) want = (V + most - 1) / most;
+  if (V > 2 * most && want < (V + most - 1) / most) want = (V + most - 1) / most;
   if (want > MAX_PARTS) want = MAX_PARTS;
   LogprobSplit s;
   s.part = (int)(((V + want - 1) / want + E - 1) / E * E);
@@ -427,12 +429,14 @@ static LogprobSplit logprob_split(int64_t rows, int V, int dtype) {
 }
 
 template <typename T>
-void logprobs_launch(const LogprobParams& p, int pieces, unsigned grid, hipStream_t st) {      // (16384 elements: 8 pieces of bf16, 16 of f32)
+void logprobs_launch(const LogprobParams& p, int pieces, unsigned grid, hipStream_t st) {
+  constexpr int MOST = 32768 / (256 * LV<T>::E);           // pieces of a thread in the longest whole row: 16 of bf16, 32 of f32
   if (pieces <= 1) token_logprobs_kernel<T, 1><<<grid, 256, 0, st>>>(p);
   else if (pieces <= 2) token_logprobs_kernel<T, 2><<<grid, 256, 0, st>>>(p);
   else if (pieces <= 4) token_logprobs_kernel<T, 4><<<grid, 256, 0, st>>>(p);
-  else if (pieces <= 8 || sizeof(T) == 2) token_logprobs_kernel<T, 8><<<grid, 256, 0, st>>>(p);
-  else token_logprobs_kernel<T, sizeof(T) == 2 ? 8 : 16><<<grid, 256, 0, st>>>(p);
+  else if (pieces <= 8) token_logprobs_kernel<T, 8><<<grid, 256, 0, st>>>(p);
+  else if (pieces <= 16) token_logprobs_kernel<T, 16><<<grid, 256, 0, st>>>(p);
+  else token_logprobs_kernel<T, MOST><<<grid, 256, 0, st>>>(p);
 }
 
 }  // namespace

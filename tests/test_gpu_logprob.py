@@ -96,7 +96,7 @@ def test_forward_over_sizes(K, rows, V, dtype):
 
 
 @pytest.mark.parametrize("kind", ["plain", "ties", "equal", "sorted", "few"])
-@pytest.mark.parametrize("rows,V", [(1, 16384), (1, 16385), (1, 17000), (3, 20000), (2, 45000), (100, 33000), (1, 1 << 20)])
+@pytest.mark.parametrize("rows,V", [(1, 16384), (1, 16385), (1, 32768), (1, 32769), (3, 33001), (2, 45000), (130, 32801), (1, 1 << 20)])
 def test_alternatives_joined_from_parts(K, rows, V, kind):
     """Rows cut into 2 .. 64 parts, fewer and more than the alternatives that are asked for."""
     x = make_logits(rows, V, torch.float32, kind, seed=V)
