@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(AppendParams p) {
 // K goes from memory straight into operand registers (lane: token l & 15, 16 bytes of its row).  bf16: V rows go through LDS, because
 // their operand needs 8 tokens of one dim per lane (ds_read_b64_tr_b16); f32: the 16x16x4 product takes ONE token per lane, so 16-byte
 // pieces of V rows are operands as they come and nothing passes through LDS.  The waves never wait for each other inside the loop.
-constexpr int MIN_PART = 128;      // tokens: one tile for each wave
+constexpr int MIN_PART = 128;      // tokens: a tile for each wave; parts are multiples of it
 
 __host__ __device__ __forceinline__ int part_tokens(int len, int nsplit) {
   const int even = (int)(((int64_t)len + nsplit - 1) / nsplit), p = (even + MIN_PART - 1) / MIN_PART * MIN_PART;
@@ -742,15 +742,20 @@ static int paged_attention_check(const NstPagedAttnDesc* d) {
   return NST_OK;
 }
 
-// How many parts a request is cut into at most: 1024 workgroups (four for a CU), and parts of at most 2048 tokens, or the last long requests
-// of a ragged batch run alone (64 requests of 1 .. 8192 tokens: 240 us with 1024 workgroups alone, 226 us so; parts half as long
-// 230 us), but none below MIN_PART.
+// How many parts a request is cut into at most.
+//   768 workgroups: what the chip holds at once (three for a CU at 128 .. 168 registers).  24 x 8 float32 heads of up to 2047 tokens: 512 / 768
+//     / 1024 / 2048 workgroups 36.7 / 32.4 / 34.0 / 35.3 us.
+//   Parts of at most 2048 tokens, or the last long requests of a ragged batch run alone (64 requests of 1 .. 8192 tokens, 8 heads: 240 us
+//     without this bound, 223 us with it, 230 us with half of it), and of at least 256.
+//   Up to 512 tokens a request stays whole (16 x 8 heads: 10.3 us, in parts with the second launch 12.1 us, and a launch less for the host),
+//     up to 1024 where there are 128 rows of heads or more (64 x 4: 14.0 against 18.7 us; 8 x 4: 18.3 against 11.6 us, so not for fewer).
 static int paged_attention_splits(const NstPagedAttnDesc* d) {
   const int64_t cap = (int64_t)d->max_pages * d->pool.page_size, bound = d->max_len > 0 && d->max_len < cap ? d->max_len : cap;
   const int64_t units = (int64_t)d->B * d->Hkv * ((d->H / d->Hkv + 15) / 16);
-  const int64_t most = (bound + MIN_PART - 1) / MIN_PART, few = (1024 + units - 1) / units, ragged = (bound + 2047) / 2048;
+  if (bound <= 512 || (bound <= 1024 && units >= 128)) return 1;
+  const int64_t most = (bound + 255) / 256, few = (768 + units - 1) / units, ragged = (bound + 2047) / 2048;
   const int64_t want = few > ragged ? few : ragged, n = want < most ? want : most;
-  return (int)(n < 1 ? 1 : n > MAX_SPLITS ? MAX_SPLITS : n);
+  return (int)(n > MAX_SPLITS ? MAX_SPLITS : n);
 }
 
 static int64_t paged_attention_ml_bytes(const NstPagedAttnDesc* d, int nsplit) {      // (the outputs behind it start 16-byte aligned)
