@@ -103,10 +103,11 @@ class NstPagedPool(C.Structure):
 
 
 class NstPagedAttnDesc(C.Structure):
+    # (the pool is a member structure of the header's; its fields follow at the same offsets, so that one call fills everything)
     _fields_ = [("B", C.c_int), ("H", C.c_int), ("Hkv", C.c_int), ("dh", C.c_int), ("max_pages", C.c_int), ("max_len", C.c_int),
                 ("scale", C.c_float), ("reserved", C.c_int),
                 ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64), ("o_row_stride", C.c_int64), ("o_head_stride", C.c_int64),
-                ("table_stride", C.c_int64), ("pool", NstPagedPool)]
+                ("table_stride", C.c_int64)] + NstPagedPool._fields_[:3] + [("pool_reserved", C.c_int)] + NstPagedPool._fields_[4:]
 
 
 _P, _I, _L, _F, _U64 = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_uint64

@@ -89,8 +89,11 @@ __device__ __forceinline__ void write_top(const LogprobParams& p, int64_t row, i
   p.top_logp[row * p.top_n + rank] = key_value(key) - lse;
 }
 
-// One workgroup holds a part of a row (up to 256 * E * NV elements) in registers: every load is requested before the first is used and
+// One workgroup holds a row, or a part of one (up to 256 * E * NV elements), in registers: every load is requested before the first is used and
 // the logits are read once, for the statistics and for the alternatives.
+// Bound by memory where there are rows enough (9600 x 8008 bf16: 27 us, 5.6 TB/s; an exponential and six more vector operations per element
+// are 77 % of the time it takes to arrive, so not much closer), else by the latency of read -> maximum -> sum -> threshold -> ranking: 128 x
+// 8008 bf16 with six alternatives 6.8 us, 4 x 128000 float32 with twenty 6.2 us and 5.5 us for the join.
 // Alternatives: the top_n-th largest of the 256 threads' maxima (found by bisection over its bits) is a value that at least top_n
 // elements reach, so only elements from it on are candidates -- a few more than top_n for ordinary rows; they are collected in LDS and ranked by
 // counting.  Rows where too many elements tie at that value take the ties in index order; what overflows even then, and rows with NaN, fall
@@ -363,6 +366,8 @@ __global__ void __launch_bounds__(256) token_logprobs_join_kernel(LogprobParams 
   }
 }
 
+// One read and one write of a row's length: 9600 x 8008 bf16 48 us, 6.4 TB/s (part of the logits still lie in the last-level cache when the
+// gradient follows the forward pass).  Each thread owns four 16-byte pieces, all requested before the row's scalars are used.
 constexpr int BWD_PIECES = 4;      // 16-byte pieces of a thread
 
 template <typename T>

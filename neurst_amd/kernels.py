@@ -852,17 +852,18 @@ def paged_attention(q, k_pool, v_pool, block_table, seq_lens, scale=None, max_le
     out = torch.empty(B, H, dh, dtype=q.dtype, device=dev)
     lse = torch.empty(B, H, dtype=_F32, device=dev) if return_lse else None
     desc = NstPagedAttnDesc(B, H, ps[2], dh, block_table.shape[1], max_len or 0, dh ** -0.5 if scale is None else scale, 0, qs[0], qs[1],
-                            H * dh, dh, stride, pool)      # (a tuple fills the nested structure)
+                            H * dh, dh, stride, *pool)
     d = C.byref(desc)
     nbytes = lib.nst_paged_attention_workspace_bytes(d)
     if nbytes < 0:
         check(nbytes, "paged_attention", launches=False)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None      # (of its own: two graphs never share it)
-    ev = PROBE.begin("paged_attention")
+    ev = PROBE.begin("paged_attention") if PROBE.names else None
     check(lib.nst_paged_attention(d, q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
                                   out.data_ptr(), lse.data_ptr() if return_lse else None, ws.data_ptr() if nbytes else None, nbytes,
                                   _stream()), "paged_attention")
-    PROBE.end(ev)
+    if ev is not None:
+        PROBE.end(ev)
     return (out, lse) if return_lse else out
 
 

@@ -18,6 +18,8 @@ class PagedKVCache(object):
     def __init__(self, num_layers, rows, num_heads, head_dim, max_length, page_size, dtype, device, static=False):
         if page_size < 1 or max_length < 1:
             raise ValueError(f"a paged cache needs pages and rows of at least one token, got {page_size} and {max_length}")
+        if head_dim > 256:
+            raise ValueError(f"the attention over pages takes heads of up to 256 elements, got {head_dim}")
         self.rows, self.page_size, self.max_length, self.static = rows, int(page_size), int(max_length), bool(static)
         self.width = -(-self.max_length // self.page_size)             # pages of a row
         pages = rows * (self.width + 1)                                # every row filled to the end, and one spare page each

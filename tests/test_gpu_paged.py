@@ -154,6 +154,17 @@ def test_attention_split_over_the_length_and_over_many_requests(K, B, lens_hi):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dh", [1, 20, 40, 64, 100, 128, 200, 256])
+@pytest.mark.parametrize("max_len", [600, 5000])
+def test_attention_joins_parts_of_every_head_size(K, max_len, dh, dtype):
+    """3 and 20 parts at most: both forms of the join, and requests that fill one part or none of them."""
+    lens = [600, 0, 5, 257, 128, 513]
+    k, v, table, ln = make_cache(lens, 16, 2, dh, dtype, seed=dh, width=max_len // 16 + 1)
+    q = torch.randn(len(lens), 6, dh, generator=gen(2)).to(dtype)
+    run_attention(K, q, k, v, table, ln, max_len=max_len)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_attention_reads_strided_operands(K, dtype):
     lens = [50, 17, 0, 90]
     H, Hk, dh = 4, 2, 48

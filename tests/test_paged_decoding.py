@@ -79,6 +79,8 @@ def test_paged_cache_of_rows_with_different_lengths(cpu_kernels):
         cache.extend(torch.full((4,), 3, dtype=torch.int32), longest=3)
     with pytest.raises(ValueError, match="at least one token"):
         PagedKVCache(1, 1, 1, 8, 4, 0, torch.float32, "cpu")
+    with pytest.raises(ValueError, match="up to 256"):
+        PagedKVCache(1, 1, 1, 300, 4, 2, torch.float32, "cpu")
 
 
 @pytest.mark.parametrize("beam,top_k,alpha,min_len,enable_unk", [(1, 1, 0.6, 0, False), (4, 4, 1.0, 0, False), (3, 2, -1.0, 0, True),

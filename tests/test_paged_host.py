@@ -23,6 +23,9 @@ def i32(a):
 
 def test_descriptor_layouts():
     assert C.sizeof(_lib.NstPagedPool) == 64 and C.sizeof(_lib.NstPagedAttnDesc) == 136
+    for f in _lib.NstPagedPool._fields_:
+        if f[0] != "reserved":
+            assert getattr(_lib.NstPagedAttnDesc, f[0]).offset == 72 + getattr(_lib.NstPagedPool, f[0]).offset
 
 
 def plan(B=1, stride=4, max_pages=4, n_free=1, page_size=4, max_tokens=1, cursor_out=8192, seq=12288, free=4096, slots=4096, cached=4096):
@@ -38,14 +41,11 @@ def test_plan_refuses(kw, text):
 
 
 def attn(**kw):
-    pool = _lib.NstPagedPool(8, 16, _lib.NST_BF16, 0, 1024, 64, 64, 1024, 64, 64)
-    d = _lib.NstPagedAttnDesc(2, 4, 2, 64, 4, 0, 0.125, 0, 256, 64, 256, 64, 4, pool)
+    d = _lib.NstPagedAttnDesc(2, 4, 2, 64, 4, 0, 0.125, 0, 256, 64, 256, 64, 4, 8, 16, _lib.NST_BF16, 0, 1024, 64, 64, 1024, 64, 64)
     ptr = dict(q=4096, k=4096, v=4096, table=4096, lens=4096, out=4096)
     for n, v in kw.items():
         if n in ptr:
             ptr[n] = v
-        elif hasattr(pool, n):
-            setattr(d.pool, n, v)
         else:
             setattr(d, n, v)
     rc = L.nst_paged_attention(C.byref(d), ptr["q"], ptr["k"], ptr["v"], ptr["table"], ptr["lens"], ptr["out"], None, None, 0, None)
