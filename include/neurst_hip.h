@@ -619,7 +619,8 @@ int nst_paged_append(const void* k, const void* v, int64_t tokens, int kv_heads,
  *   out[b, h] = sum_{t < seq_lens[b]} softmax_t(scale * q[b, h] . k_t[h']) v_t[h'],   h' = h / (H / Hkv)
  * lse (nullable) [B, H] f32 = log-sum-exp of the scaled scores.  A request with no (valid) token gets out = 0, lse = -inf.  Lengths are
  * clamped to [0, max_pages * page_size]; tokens behind a request's length are not read.  Scores, softmax statistics and the sums
- * are f32; with NST_BF16 the probabilities are rounded to bf16 for the product with v.
+ * are f32; with NST_BF16 a probability enters the product with v as the sum of two bf16 numbers (2^-16 of itself; an
+ * infinite v of a token in range therefore gives NaN).
  * max_len: a bound of seq_lens that the host knows (0: max_pages * page_size).  It only chooses how the work is split; a longer
  * request is still attended over in full. */
 typedef struct {

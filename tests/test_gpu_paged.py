@@ -4,8 +4,9 @@ end inside every tile, heads of odd sizes, strided operands, entries outside the
 
 Tolerances.  Everything that only moves data or counts is compared for equality.  The attention sums n terms in f32 (u = 2^-24): a score
 is off by at most u (dh + 4) scale sum|q||k| (products and sum) + 3 u |s| (scale and log2 e), which scales a weight by twice that; the two
-sums add at most 2 (n + 8) u.  With bf16 every weight is rounded (2^-8 of itself) and so is the output (2^-8 of itself):
-    |o - o64| <= [2 ds + 2 (n + 8) u] sum p|v|   +   bf16: 2^-8 sum p|v| + 2^-8 |o64|,   f32: u |o64|
+sums add at most 2 (n + 8) u.  With bf16 a weight is the sum of two roundings (off by 2^-8 of 2^-8 of itself) and the output is rounded
+(2^-8 of itself):
+    |o - o64| <= [2 ds + 2 (n + 8) u] sum p|v|   +   bf16: 2^-16 sum p|v| + 2^-8 |o64|,   f32: u |o64|
 """
 import math
 
@@ -79,7 +80,7 @@ def attention_reference(q, k_pool, v_pool, table, lens, scale):
             ds = float((U * (dh + 4) * abs(scale) * (kh.abs() @ qh.abs()) + 3 * U * s.abs()).max())
             mag = p @ vh.abs()
             out[b, h], lse[b, h] = p @ vh, torch.logsumexp(s, 0)
-            tol[b, h] = (2 * ds + 2 * (page.numel() + 8) * U + half) * mag + max(half, U) * out[b, h].abs()
+            tol[b, h] = (2 * ds + 2 * (page.numel() + 8) * U + half * half) * mag + max(half, U) * out[b, h].abs()
     return out, lse, tol
 
 
