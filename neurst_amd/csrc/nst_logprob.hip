@@ -211,7 +211,8 @@ __global__ void __launch_bounds__(256) token_logprobs_kernel(LogprobParams p) {
     uint32_t tau = 0;
     for (int bit = 31; bit >= 32 - bits; --bit) {
       const uint32_t probe = tau | (1u << bit);
-      const int cnt = __popcll(__ballot(a >= probe)) + __popcll(__ballot(b >= probe)) + __popcll(__ballot(c >= probe)) + __popcll(__ballot(d >= probe));
+      const int cnt = __popcll(__ballot(a >= probe)) + __popcll(__ballot(b >= probe)) + __popcll(__ballot(c >= probe)) +
+                      __popcll(__ballot(d >= probe));
       if (cnt >= want) tau = probe;
     }
     return tau;
@@ -510,9 +511,11 @@ extern "C" int nst_token_logprobs_bwd(const void* logits, const int64_t* tokens,
   hipStream_t st = (hipStream_t)stream;
   const unsigned grid = (unsigned)(rows * chunks);
   if (dtype == NST_BF16)
-    token_logprobs_bwd_kernel<bf16_t><<<grid, 256, 0, st>>>((const bf16_t*)logits, tokens, lse, entropy, dlogp, dentropy, (bf16_t*)dlogits, V, ldl, ldd, chunks);
+    token_logprobs_bwd_kernel<bf16_t><<<grid, 256, 0, st>>>((const bf16_t*)logits, tokens, lse, entropy, dlogp, dentropy,
+                                                            (bf16_t*)dlogits, V, ldl, ldd, chunks);
   else
-    token_logprobs_bwd_kernel<float><<<grid, 256, 0, st>>>((const float*)logits, tokens, lse, entropy, dlogp, dentropy, (float*)dlogits, V, ldl, ldd, chunks);
+    token_logprobs_bwd_kernel<float><<<grid, 256, 0, st>>>((const float*)logits, tokens, lse, entropy, dlogp, dentropy, (float*)dlogits, V,
+                                                           ldl, ldd, chunks);
   NST_CHECK_LAUNCH("nst_token_logprobs_bwd");
   return NST_OK;
 }

@@ -245,3 +245,10 @@ def test_captured_forward_and_gradient(K):
         torch.cuda.synchronize()
         for p, q in zip(got, want):
             assert torch.equal(p, q), i
+
+
+def test_calls_with_nothing_in_them(K):
+    x, tokens = torch.zeros(0, 30, device=DEV), torch.zeros(0, dtype=torch.int64, device=DEV)
+    logp, entropy, lse, top_logp, top_ids = K.token_logprobs(x, tokens, 3)
+    assert logp.shape == entropy.shape == lse.shape == (0,) and top_logp.shape == top_ids.shape == (0, 3)
+    assert K.token_logprobs_bwd(x, tokens, lse, entropy, logp, entropy).shape == (0, 30)

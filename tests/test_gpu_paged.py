@@ -453,3 +453,47 @@ def test_calls_on_another_stream(K):
         b = K.paged_attention(q, kd, vd, td, ld)
     side.synchronize()
     assert torch.equal(a, b)
+
+
+def test_calls_with_nothing_in_them(K):
+    z = lambda *shape, dt=torch.int32: torch.zeros(*shape, dtype=dt, device=DEV)      # noqa: E731
+    pool = z(4, 16, 2, 64, dt=torch.float32)
+    assert K.paged_attention(z(0, 4, 64, dt=torch.float32), pool, pool, z(0, 3), z(0)).shape == (0, 4, 64)
+    K.paged_append(z(0, 2, 64, dt=torch.float32), z(0, 2, 64, dt=torch.float32), pool, pool, z(0, dt=torch.int64))
+    slots, lens, cu, cursor = K.paged_plan(z(0), z(0), z(0, 3), z(5), i32([2]).to(DEV), 16, 4)
+    assert slots.tolist() == [-1] * 4 and lens.numel() == 0 and cu.tolist() == [0] and cursor.tolist() == [2]
+    slots, lens, cu, cursor = K.paged_plan(i32([3, 0]).to(DEV), z(2), z(2, 3), z(0), z(1), 16, 0)
+    assert slots.numel() == 0 and lens.tolist() == [3, 0] and cu.tolist() == [0, 0, 0] and cursor.tolist() == [0]
+    t, s = K.paged_reorder(z(2, 4, 16, 8, dt=torch.float32), z(0, 3), z(0), z(0, dt=torch.int64), z(0))
+    assert t.shape == (0, 3) and s.shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_over_a_pool_without_pages(K, dtype):
+    """Nothing exists that a table could name: no row is read, every output is 0 -- whole requests and requests in parts."""
+    pool = torch.zeros(0, 16, 2, 64, dtype=dtype, device=DEV)
+    q = torch.randn(3, 4, 64, generator=gen(0)).to(dtype).to(DEV)
+    for W in (2, 100):
+        table = torch.zeros(3, W, dtype=torch.int32, device=DEV)
+        out, lse = K.paged_attention(q, pool, pool, table, i32([W * 16, 5, 0]).to(DEV), return_lse=True)
+        assert (out == 0).all() and torch.isinf(lse).all() and (lse < 0).all()
+
+
+def test_two_calls_at_once(K):
+    """Long requests on two streams at the same time: each call has scratch of its own."""
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    cases = []
+    for i in range(2):
+        k, v, table, ln = make_cache([3000, 4000 - 100 * i, 1], 16, 2, 64, torch.bfloat16, seed=i)
+        q = torch.randn(3, 4, 64, generator=gen(6 + i)).to(torch.bfloat16)
+        cases.append([t.to(DEV) for t in (q, k, v, table, ln)])
+    want = [K.paged_attention(*c) for c in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(sides[i]):
+                got[i].append(K.paged_attention(*cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])

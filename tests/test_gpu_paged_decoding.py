@@ -65,3 +65,22 @@ def test_entropy_regularized_training_step(dtype, tol):
     statistics that agree to 1e-6; the rest of the backward pass is the same linear map with the same roundings of other values
     (another 2^-8 on each side)."""
     run_entropy_training(DEV, dtype, tol)
+
+
+def test_entropy_regularized_training_replays_from_a_graph():
+    """Graph replay equals eager steps with this criterion too (float32, no dropout: the embedding gradient's atomics leave last-bit
+    differences, 1e-5 as in the test of the label-smoothed criterion)."""
+    from test_gpu_graph import _batch, _setup
+    from neurst_amd.criterions import build_criterion
+    batches, res = [_batch(300 + i) for i in range(5)], {}
+    for use_graph in (False, True):
+        model, step, _ = _setup("float32", 0.0, use_graph)
+        step.criterion = build_criterion({"criterion.class": "entropy_regularized_cross_entropy", "criterion.params": {"entropy_weight": 0.1}})
+        losses = []
+        for b in batches:
+            losses.append(float(step(b)))
+            torch.cuda.synchronize()
+        res[use_graph] = losses
+        assert step.replays == (len(batches) - 1 if use_graph else 0)
+    for a, b in zip(res[False], res[True]):
+        assert abs(a - b) <= 1e-5 * max(1.0, abs(a)), res
