@@ -260,7 +260,7 @@ struct PagedAttnParams {
   uint32_t k_page, k_tok, v_page, v_tok;                            // elements, below 2^31
   int64_t k_head, v_head;
   float scale_log2;
-  int nsplit, qchunks;
+  int nsplit, qchunks, by_xcd;
   FastDiv page;
   float* part_ml;          // [B * H][nsplit][2]: maximum and sum of a part
   float* part_o;           // [B * H][nsplit][dh rounded up to 4]: its output
@@ -307,7 +307,14 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnParams p) {
   __shared__ float s_ml[2][4][16];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, lc = lane & 15;
   const int heads = p.Hkv * p.qchunks;
-  const int hq = blockIdx.x % heads, rest = blockIdx.x / heads, split = rest % p.nsplit, b = rest / p.nsplit;
+  int hq = blockIdx.x % heads, rest = blockIdx.x / heads;
+  if (p.by_xcd) {          // (see paged_attention_by_xcd)
+    const int turn = blockIdx.x >> 3;
+    hq = turn % heads;
+    rest = turn / heads * 8 + (blockIdx.x & 7);
+    if (rest >= p.B * p.nsplit) return;
+  }
+  const int split = rest % p.nsplit, b = rest / p.nsplit;
   const int hk = hq / p.qchunks, qc = hq % p.qchunks, group = p.H / p.Hkv;
   const int h0 = hk * group + qc * 16, nh = min(16, group - qc * 16);
   const int cap = p.max_pages * p.page_size;
@@ -830,6 +837,12 @@ static int paged_attention_splits(const NstPagedAttnDesc* d) {
   return (int)(n > MAX_SPLITS ? MAX_SPLITS : n);
 }
 
+// Workgroups go to the eight XCDs in turn.  All heads of a part of a request on ONE of them find in its cache what their rows share: cache lines,
+// where a head's row is not a multiple of 128 bytes (16 requests, 8 heads of 40 bf16: 90 -> 57 us; 32 requests, 8 heads of 32: 88 -> 54 us),
+// and whole rows, where more than 16 query heads read them (128 over one, 256 wide: 314 -> 221 us); others do not care (64 x 8 heads of 128:
+// 396, 392 us).  From 64 parts on: below, eight XCDs would have unequally many.
+static bool paged_attention_by_xcd(int64_t parts) { return parts >= 64; }
+
 static int64_t paged_attention_ml_bytes(const NstPagedAttnDesc* d, int nsplit) {      // (the outputs behind it start 16-byte aligned)
   return ((int64_t)d->B * d->H * nsplit * 8 + 15) / 16 * 16;
 }
@@ -878,7 +891,9 @@ extern "C" int nst_paged_attention(const NstPagedAttnDesc* d, const void* q, con
     p.part_ml = (float*)workspace;
     p.part_o = (float*)((char*)workspace + paged_attention_ml_bytes(d, p.nsplit));
   }
-  const int64_t blocks = (int64_t)d->B * d->Hkv * p.qchunks * p.nsplit;
+  const int64_t parts = (int64_t)d->B * p.nsplit;
+  p.by_xcd = paged_attention_by_xcd(parts);
+  const int64_t blocks = (p.by_xcd ? (parts + 7) / 8 * 8 : parts) * d->Hkv * p.qchunks;
   NST_CHECK_ARG(blocks <= 0x7fffffffLL, "nst_paged_attention: %lld workgroups", (long long)blocks);
   const int es = nst_dtype_size(pl.dtype);
   bool vec = nst_aligned16(q) && nst_aligned16(p.k) && nst_aligned16(p.v) && (d->dh * es) % 16 == 0;
