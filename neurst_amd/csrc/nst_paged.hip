@@ -907,8 +907,9 @@ extern "C" int nst_paged_attention(const NstPagedAttnDesc* d, const void* q, con
     else if (d->dh <= 128) paged_attn_launch<bf16_t, 128, 2>(p, vec, grid, st);
     else paged_attn_launch<bf16_t, 256, 2>(p, vec, grid, st);
   } else {
+    // (tiles of 16 tokens from 65 on: with 32 a wave needs more than 256 registers and a SIMD holds one; 13 x 8 heads of 80: 78, 61 us)
     if (d->dh <= 64) paged_attn_launch<float, 64, 2>(p, vec, grid, st);
-    else if (d->dh <= 128) paged_attn_launch<float, 128, 2>(p, vec, grid, st);
+    else if (d->dh <= 128) paged_attn_launch<float, 128, 1>(p, vec, grid, st);
     else paged_attn_launch<float, 256, 1>(p, vec, grid, st);
   }
   if (p.nsplit > 1) {
