@@ -826,12 +826,14 @@ static int paged_attention_check(const NstPagedAttnDesc* d) {
 //     / 1024 / 2048 workgroups 36.7 / 32.4 / 34.0 / 35.3 us.
 //   Parts of at most 2048 tokens, or the last long requests of a ragged batch run alone (64 requests of 1 .. 8192 tokens, 8 heads: 240 us
 //     without this bound, 223 us with it, 230 us with half of it), and of at least 256.
-//   Up to 512 tokens a request stays whole (16 x 8 heads: 10.3 us, in parts with the second launch 12.1 us, and a launch less for the host),
+//   Up to 512 tokens a request stays whole (16 x 8 heads: 10.3 us, in parts with the second launch 12.1 us, and a launch less for the host;
+//     up to 256 of float32 with tiles of 16 tokens: 29 x 2 heads of 80, 512 tokens 24.9 us whole, 18.8 in parts),
 //     up to 1024 where there are 128 rows of heads or more (64 x 4: 14.0 against 18.7 us; 8 x 4: 18.3 against 11.6 us, so not for fewer).
 static int paged_attention_splits(const NstPagedAttnDesc* d) {
   const int64_t cap = (int64_t)d->max_pages * d->pool.page_size, bound = d->max_len > 0 && d->max_len < cap ? d->max_len : cap;
   const int64_t units = (int64_t)d->B * d->Hkv * ((d->H / d->Hkv + 15) / 16);
-  if (bound <= 512 || (bound <= 1024 && units >= 128)) return 1;
+  const int64_t whole = d->pool.dtype == NST_F32 && d->dh > 64 ? 256 : 512;
+  if (bound <= whole || (bound <= 1024 && units >= 128)) return 1;
   const int64_t most = (bound + 255) / 256, few = (768 + units - 1) / units, ragged = (bound + 2047) / 2048;
   const int64_t want = few > ragged ? few : ragged, n = want < most ? want : most;
   return (int)(n > MAX_SPLITS ? MAX_SPLITS : n);
