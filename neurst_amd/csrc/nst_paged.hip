@@ -136,7 +136,6 @@ __global__ void __launch_bounds__(256) paged_plan_kernel(PlanParams p) {
     }
     return lo;
   };
-  auto free_page = [&](int64_t at) __attribute__((always_inline)) { return at < p.n_free ? p.free_pages[at] : -1; };
   if (blockIdx.y == 0) {
     if (tid < nb) {
       int64_t got = (int64_t)p.n_free - (page_base + page_off[tid]);
@@ -146,8 +145,9 @@ __global__ void __launch_bounds__(256) paged_plan_kernel(PlanParams p) {
       p.seq_lens[b0 + tid] = (int)(want < cap ? want : cap);
       p.cu_new[b0 + tid] = (int)(tok_base + tok_off[tid]);
     }
-    for (int i = tid; i < n_page; i += 256) {
-      const int r = find(page_off, i), page = free_page(page_base + i);
+    const int64_t left = p.n_free - page_base;             // pages behind these do not exist: a senseless length costs no walk
+    for (int64_t i = tid; i < n_page && i < left; i += 256) {
+      const int r = find(page_off, (int)i), page = p.free_pages[page_base + i];
       if (page >= 0) p.table[(int64_t)(b0 + r) * p.table_stride + s_held[r] + (i - page_off[r])] = page;
     }
   }

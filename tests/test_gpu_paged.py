@@ -291,6 +291,18 @@ def test_plan_with_too_few_pages_and_full_table_rows(K, n_free, cursor):
     assert torch.equal(t_dev.cpu(), t_ref)
 
 
+def test_plan_with_senseless_lengths_ends(K):
+    """Lengths near 2^31 in every request, pages of one token in a table row of 2^20: what cannot be served costs nothing."""
+    B, W = 70, 1 << 20
+    big = 2 ** 31 - 1
+    cached, new = i32([big, -big - 1, 5] + [0] * (B - 3)), i32([big] * B)
+    table = torch.full((B, W), -1, dtype=torch.int32, device=DEV)
+    slots, lens, cu, cursor = K.paged_plan(cached.to(DEV), new.to(DEV), table, torch.arange(9, dtype=torch.int32, device=DEV), i32([4]).to(DEV), 1, 20)
+    # request 0 is full; the five free pages go to request 1, whose tokens stand behind request 0's and past the twenty slots
+    assert slots.tolist() == [-1] * 20 and cursor.tolist() == [9] and lens.tolist() == [W, 0, 5] + [0] * (B - 3)
+    assert table[1, :6].tolist() == [4, 5, 6, 7, 8, -1]
+
+
 # ------------------------------------------------------------------------------------------------ append
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("T,Hk,dh,ps", [(1, 1, 1, 1), (5, 2, 5, 3), (128, 4, 64, 16), (1000, 8, 40, 24), (333, 1, 256, 7)])
