@@ -8,6 +8,7 @@ backward pass has finished the layers they cover (neurst_amd/training/distribute
 """
 import collections
 import contextlib
+import gc
 import math
 import os
 
@@ -347,6 +348,24 @@ def make_stream(device, priority_class):
                                          if os.environ.get("GPU_MAX_HW_QUEUES") == "1" else ""))
         return torch.cuda.Stream(device)
     return torch.cuda.ExternalStream(handle.value, device=device)   # lives as long as the process
+
+
+@contextlib.contextmanager
+def quiet_capture(device=None):
+    """Around the capture of a HIP graph: no destructor of a device object may run while a stream is being captured.  Destroying a captured
+    graph waits for the device, which a capture forbids, and the error leaves a destructor: the process ends.  So garbage that earlier
+    work left in reference cycles (an older step's or model's graphs, events, streams) is collected on entry, on an idle device, and the
+    cyclic collector stays off until the capture has ended; torch.cuda.graph() does neither.  (Seen when a model with captured
+    graphs was dropped before another one captured its own in the same process.)"""
+    torch.cuda.synchronize(device)
+    gc.collect()
+    was_on = gc.isenabled()
+    gc.disable()
+    try:
+        yield
+    finally:
+        if was_on:
+            gc.enable()
 
 
 class Runtime(object):

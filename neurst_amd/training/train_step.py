@@ -22,6 +22,7 @@ import warnings
 import torch
 
 from neurst_amd import _lib
+from neurst_amd.runtime import quiet_capture
 
 
 class _Segment(object):
@@ -347,37 +348,26 @@ class TrainStep(object):
         sc = _StepCapture(rt, cap.pool, stream, self._side_stream)
         if red is not None:
             red.capture_cut = sc.cut_for_bucket
-        # No destructor of a device object may run while the step is being captured: garbage left by earlier work (an older
-        # TrainStep's graphs, events, streams in reference cycles) is collected NOW, on an idle device, and the cyclic collector
-        # stays off until the capture has ended -- what torch.cuda.graph() does on entry; a collection that freed a captured
-        # graph of an earlier model in the middle of this capture aborted the process (seen when tests/test_gpu_graph.py ran
-        # behind tests/test_gpu_model.py in one interpreter).
-        import gc
-        torch.cuda.synchronize(rt.device)
-        gc.collect()
-        gc_was_on = gc.isenabled()
-        gc.disable()
-        rt.capture = sc
-        try:
-            with torch.cuda.stream(stream):
-                sc.begin()
-                loss = self._body(full, lr_t_dev=self._lr_dev)
-                with rt.bound():
-                    K.dropout_seed_offset_add(1)
-                cap.loss = loss
-                sc.finish()
-        finally:
-            if gc_was_on:
-                gc.enable()
-            rt.capture = None
-            if red is not None:
-                red.capture_cut = None
-            if sc.cur is not None:   # an exception inside the capture: leave capture mode
-                try:
-                    sc.cur.main.capture_end()
-                except Exception:
-                    pass
-                rt.drop_pending_wgrads()   # nothing of the aborted step may run inside the next one's grouped launch
+        with quiet_capture(rt.device):
+            rt.capture = sc
+            try:
+                with torch.cuda.stream(stream):
+                    sc.begin()
+                    loss = self._body(full, lr_t_dev=self._lr_dev)
+                    with rt.bound():
+                        K.dropout_seed_offset_add(1)
+                    cap.loss = loss
+                    sc.finish()
+            finally:
+                rt.capture = None
+                if red is not None:
+                    red.capture_cut = None
+                if sc.cur is not None:   # an exception inside the capture: leave capture mode
+                    try:
+                        sc.cur.main.capture_end()
+                    except Exception:
+                        pass
+                    rt.drop_pending_wgrads()   # nothing of the aborted step may run inside the next one's grouped launch
         torch.cuda.current_stream(rt.device).wait_stream(stream)
         cap.segments, cap.keep = sc.segments, sc.keep
         return cap

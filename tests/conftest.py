@@ -1,3 +1,4 @@
+import gc
 import os
 import sys
 
@@ -15,6 +16,13 @@ def pytest_configure(config):
     # applied here, before any test touches the device -- importing neurst_amd does not do it
     from neurst_amd.runtime import configure_training_process
     configure_training_process()
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _collected():
+    """Captured graphs that earlier tests left in reference cycles go before a module's tests, some of which capture graphs by themselves:
+    one destroyed in the middle of a capture would end the process (neurst_amd.runtime.quiet_capture)."""
+    gc.collect()
 
 
 def load_golden(name):

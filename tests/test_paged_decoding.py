@@ -1,6 +1,10 @@
 """Where the paged caches and the token log probabilities are used: the decoder's paged self-attention cache under the beam search, the search
 that ranks only the likeliest symbols, and the cross entropy with an entropy term.  Host logic over the float64 restatement of the kernels'
 contracts; the same calls on the device are in test_gpu_paged_decoding.py."""
+import contextlib
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -180,3 +184,81 @@ def run_entropy_training(device, dtype, tol):
 def test_entropy_regularized_training_of_the_model(cpu_kernels):
     # f32 results of float64 arithmetic on both sides: the two d(logits) differ by a rounding (2^-24) each, carried linearly
     run_entropy_training("cpu", "float32", 1e-5)
+
+
+# ------------------------------------------------------------------------------------------------ captured decoding steps
+class _GraphStub(object):
+    """In the place of a HIP graph: capturing runs the step once, replaying does nothing (what the first batch of a session needs)."""
+    collector_on = []
+
+    def __init__(self):
+        self.in_cycle = self                                     # like everything that waits for the cyclic collector
+
+    def pool(self):
+        return 1
+
+    def replay(self):
+        pass
+
+
+@contextlib.contextmanager
+def _capture_stub(graph, pool=None, **kwargs):
+    _GraphStub.collector_on.append(gc.isenabled())
+    yield
+
+
+@pytest.fixture
+def stubbed_graphs(cpu_kernels, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", _GraphStub)
+    monkeypatch.setattr(torch.cuda, "graph", _capture_stub)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: None)
+    _GraphStub.collector_on = []
+    return _GraphStub
+
+
+@pytest.mark.parametrize("page_size", [None, 4])
+def test_no_collection_runs_while_a_decoding_step_is_captured(stubbed_graphs, monkeypatch, page_size):
+    """A collection in the middle of a capture may destroy the captured graphs of a model that was dropped earlier: the process would end.
+    What is there to collect goes before the capture, and the collector comes back behind it, also behind one that fails."""
+    from neurst_amd.layers.search import BeamSearch
+    model, inputs = _toy_model(seed=11), _inputs()
+    kw = dict(beam_size=3, top_k=2, maximum_decode_length=8, page_size=page_size)
+    h0, s0 = BeamSearch(**kw)(model, inputs)
+    garbage = weakref.ref(stubbed_graphs())                      # freed by the cyclic collector alone
+    assert gc.isenabled() and garbage() is not None
+    h1, s1 = BeamSearch(use_graphs=True, **kw)(model, inputs)
+    assert torch.equal(h0, h1) and torch.equal(s0, s1)
+    assert stubbed_graphs.collector_on and not any(stubbed_graphs.collector_on) and gc.isenabled() and garbage() is None
+
+    def failing(graph, pool=None):
+        raise RuntimeError("no capture")
+    monkeypatch.setattr(torch.cuda, "graph", failing)
+    with pytest.raises(RuntimeError, match="no capture"):
+        BeamSearch(use_graphs=True, **dict(kw, maximum_decode_length=7))(model, inputs)
+    assert gc.isenabled()
+    gc.disable()
+    try:                                                         # off before: off afterwards
+        monkeypatch.setattr(torch.cuda, "graph", _capture_stub)
+        BeamSearch(use_graphs=True, **dict(kw, maximum_decode_length=6))(model, inputs)
+        assert not gc.isenabled()
+    finally:
+        gc.enable()
+
+
+@pytest.mark.parametrize("page_size", [None, 4])
+def test_a_dropped_model_takes_its_captured_steps_along(stubbed_graphs, page_size):
+    """... at once, not when the cyclic collector comes by; and the step function alone keeps its model alive."""
+    model, inputs = _toy_model(seed=11), _inputs()
+    fn, init, _ = model.get_symbols_to_logits_fn(inputs, beam_size=2, decode_padded_length=6, use_graphs=True,
+                                                 **({"page_size": page_size} if page_size else {}))
+    alive = weakref.ref(model)
+    session = weakref.ref(next(iter(model._decode_sessions.values())))
+    del model
+    logits = fn(torch.full((4,), 18), init["decoder_internal_cache"], 0)
+    assert logits.shape == (4, 20) and alive() is not None and len(session().graphs) == 1
+    gc.disable()
+    try:
+        del fn, init
+        assert alive() is None and session() is None
+    finally:
+        gc.enable()
