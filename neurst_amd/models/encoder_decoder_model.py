@@ -64,7 +64,7 @@ class _DecodeSession(object):
                 for st in cache["decoding_states"].values():
                     st["encdec_attention"].pop("kv", None)
             graph = torch.cuda.CUDAGraph()
-            with quiet_capture(), torch.cuda.graph(graph, pool=self.pool):
+            with quiet_capture(collect=not self.graphs), torch.cuda.graph(graph, pool=self.pool):
                 static_logits = eager_step(static_ids, cache, time)
             if self.pool is None:
                 self.pool = graph.pool()

@@ -351,14 +351,16 @@ def make_stream(device, priority_class):
 
 
 @contextlib.contextmanager
-def quiet_capture(device=None):
+def quiet_capture(device=None, collect=True):
     """Around the capture of a HIP graph: no destructor of a device object may run while a stream is being captured.  Destroying a captured
-    graph waits for the device, which a capture forbids, and the error leaves a destructor: the process ends.  So garbage that earlier
-    work left in reference cycles (an older step's or model's graphs, events, streams) is collected on entry, on an idle device, and the
-    cyclic collector stays off until the capture has ended; torch.cuda.graph() does neither.  (Seen when a model with captured
-    graphs was dropped before another one captured its own in the same process.)"""
+    graph waits for the device, which a capture forbids, and the error leaves a destructor: the process ends.  So the cyclic collector
+    stays off until the capture has ended; torch.cuda.graph() does not see to that.  (Seen when a model with captured graphs was
+    dropped before another one captured its own in the same process.)
+    collect: what earlier work left in reference cycles (an older step's or model's graphs, events, streams, memory) is collected on entry, on
+    an idle device.  One in front of a series of captures is enough: it takes some 50 ms."""
     torch.cuda.synchronize(device)
-    gc.collect()
+    if collect:
+        gc.collect()
     was_on = gc.isenabled()
     gc.disable()
     try:
