@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(256) token_logprobs_join_kernel(LogprobParams 
   }
   const float M = wave_max(m), mu = M == -INFINITY ? 0.f : M;
   const float d = m - mu, c = __builtin_amdgcn_exp2f(d * LOG2E);
-  t = wave_sum(c * fmaf(fmaxf(d, LOWEST), s, t));
+  t = wave_sum(fmaf(c * fmaxf(d, LOWEST), s, c * t));      // (c first: d * s overflows where a part holds nothing but large finite masks, c is 0 there)
   s = wave_sum(c * s);
   const float log_s = M == -INFINITY ? NAN : logf(s), lse = M + log_s;
   if (tid == 0) write_row<T>(p, row, lse, log_s, t / s);

@@ -252,3 +252,20 @@ def test_calls_with_nothing_in_them(K):
     logp, entropy, lse, top_logp, top_ids = K.token_logprobs(x, tokens, 3)
     assert logp.shape == entropy.shape == lse.shape == (0,) and top_logp.shape == top_ids.shape == (0, 3)
     assert K.token_logprobs_bwd(x, tokens, lse, entropy, logp, entropy).shape == (0, 30)
+
+
+# ------------------------------------------------------------------------------------------------ masks and offsets
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mask", [-1e9, -1e36, float(torch.finfo(torch.bfloat16).min), float(torch.finfo(torch.float32).min), -math.inf])
+@pytest.mark.parametrize("rows,V", [(1, 3000), (1, 40000), (4, 40000), (130, 40000), (1, 128000), (4, 128000), (130, 128000)])
+def test_parts_of_nothing_but_ruled_out_symbols(K, rows, V, mask, dtype):
+    """A short list is allowed, everything else has a large finite mask: whole parts of a row hold nothing else.  They add exactly nothing --
+    to the entropy and to the gradient that takes it, too."""
+    g = gen(V + rows)
+    x = torch.full((rows, V), mask)
+    for r in range(rows):
+        x[r, torch.randperm(V, generator=g)[:20]] = torch.randn(20, generator=g) * 2
+    x = x.to(dtype)
+    tokens = x.argmax(-1)
+    assert_forward(K, x, tokens, 6)
+    assert_backward(K, x, tokens, torch.randn(rows, generator=g), torch.randn(rows, generator=g))
