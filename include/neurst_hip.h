@@ -652,7 +652,8 @@ int nst_paged_reorder(void* pool, int planes, int64_t plane_stride, int num_page
 
 /* ------------------------------------------------------------------ log probabilities of given tokens
  * logits [rows, V] (row stride ldl elements), V <= 2^20.  One read of the logits gives, per row (f32, each output nullable):
- *   logp = log softmax(logits)[token]   (0 where the token is outside [0, V): padding),   lse = log-sum-exp,
+ *   logp = log softmax(logits)[token]   (0 where the token is outside [0, V): padding; exact to f32 rounding also where all logits are
+ *   large: what they have in common drops out before it is rounded),   lse = log-sum-exp,
  *   entropy = -sum p log p,   top_logp / top_ids [rows, top_n]: the top_n <= min(64, V) likeliest tokens in descending order
  * (tf.nn.log_softmax + tf.nn.top_k of beam_search.py:104-215).  Equal logits rank by the lower id, a NaN ranks first.  A ruled-out
  * logit (-1e9, -inf) has probability 0 and adds nothing to the entropy; a row of nothing but -inf gives NaN as softmax does.
@@ -662,7 +663,8 @@ int nst_token_logprobs_fwd(const void* logits, const int64_t* tokens, float* log
                            int64_t* top_ids, int64_t rows, int V, int64_t ldl, int top_n, int dtype, void* workspace,
                            int64_t workspace_bytes, void* stream);
 /* dlogits = dlogp * ([j = token] - p_j) - dentropy * p_j * (log p_j + entropy); dlogp, dentropy [rows] f32, each nullable; lse and entropy
- * as the forward call left them.  dlogits may be logits itself (ldd == ldl), and must not overlap it otherwise.  The alternatives
+ * as the forward call left them.  p_j = exp(logits_j - lse) from the rounded lse: off by 2^-24 |lse| of itself (6e-5 where the logits lie around
+ * 1000).  dlogits may be logits itself (ldd == ldl), and must not overlap it otherwise.  The alternatives
  * carry no gradient. */
 int nst_token_logprobs_bwd(const void* logits, const int64_t* tokens, const float* lse, const float* entropy, const float* dlogp,
                            const float* dentropy, void* dlogits, int64_t rows, int V, int64_t ldl, int64_t ldd, int dtype, void* stream);

@@ -1,7 +1,7 @@
 // Log probabilities of given tokens, entropy and top alternatives of rows of logits, and the gradient.
 //
 //   m = max_j x_j,  S = sum_j exp(x_j - m),  T = sum_j (x_j - m) exp(x_j - m)
-//   lse = m + log S        log p(token) = x_token - lse        H = -sum_j p_j log p_j = log S - T / S
+//   lse = m + log S        log p(token) = (x_token - m) - log S        H = -sum_j p_j log p_j = log S - T / S
 //   d x_j = d_logp * ([j = token] - p_j) - d_H * p_j * (log p_j + H)
 // T is summed over x - m, not over x: the terms stay small, and a ruled-out symbol (-1e9, or minus infinity) adds exactly 0.
 #include "nst_common.h"
@@ -74,19 +74,20 @@ struct LogprobParams {
   uint64_t* keys;                 //             [rows][nparts][top_n], descending, 0: none
 };
 
-// What a row's statistics give: one thread
+// What a row's statistics give: one thread.  log p is (x - m) - log S, not x - lse: lse is rounded at its own size (3e-5 at 1000), while what the
+// likely logits have in common with m drops out of x - m exactly.
 template <typename T>
-__device__ __forceinline__ void write_row(const LogprobParams& p, int64_t row, float lse, float log_s, float ratio) {
-  if (p.lse) p.lse[row] = lse;
+__device__ __forceinline__ void write_row(const LogprobParams& p, int64_t row, float m, float log_s, float ratio) {
+  if (p.lse) p.lse[row] = m + log_s;
   if (p.entropy) p.entropy[row] = log_s - ratio;
   if (p.logp) {
     const int64_t tok = p.tokens[row];
-    p.logp[row] = tok >= 0 && tok < p.V ? to_f32<T>(((const T*)p.logits)[row * p.ldl + tok]) - lse : 0.f;
+    p.logp[row] = tok >= 0 && tok < p.V ? (to_f32<T>(((const T*)p.logits)[row * p.ldl + tok]) - m) - log_s : 0.f;
   }
 }
-__device__ __forceinline__ void write_top(const LogprobParams& p, int64_t row, int rank, uint64_t key, float lse) {
+__device__ __forceinline__ void write_top(const LogprobParams& p, int64_t row, int rank, uint64_t key, float m, float log_s) {
   p.top_ids[row * p.top_n + rank] = key_index(key);
-  p.top_logp[row * p.top_n + rank] = key_value(key) - lse;
+  p.top_logp[row * p.top_n + rank] = (key_value(key) - m) - log_s;
 }
 
 // One workgroup holds a row, or a part of one (up to 256 * E * NV elements), in registers: every load is requested before the first is used and
@@ -163,10 +164,10 @@ __global__ void __launch_bounds__(256) token_logprobs_kernel(LogprobParams p) {
   s = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
   t = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
   const bool single = p.nparts == 1;
-  const float log_s = m == -INFINITY ? NAN : logf(s), lse = m + log_s;
+  const float log_s = m == -INFINITY ? NAN : logf(s);
   if (tid == 0) {
     if (single) {
-      write_row<T>(p, row, lse, log_s, t / s);
+      write_row<T>(p, row, m, log_s, t / s);
     } else {
       float* st = p.stats + (row * p.nparts + part) * 4;
       st[0] = m; st[1] = s; st[2] = t;
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(256) token_logprobs_kernel(LogprobParams p) {
   const int want = min(p.top_n, n);
   uint64_t* keys = single ? nullptr : p.keys + (row * p.nparts + part) * p.top_n;
   auto emit = [&](int rank, uint64_t key) __attribute__((always_inline)) {
-    if (single) write_top(p, row, rank, key, lse);
+    if (single) write_top(p, row, rank, key, m, log_s);
     else keys[rank] = key;
   };
   if (!single)
@@ -331,8 +332,8 @@ __global__ void __launch_bounds__(256) token_logprobs_join_kernel(LogprobParams 
   const float d = m - mu, c = __builtin_amdgcn_exp2f(d * LOG2E);
   t = wave_sum(fmaf(c * fmaxf(d, LOWEST), s, c * t));      // (c first: d * s overflows where a part holds nothing but large finite masks, c is 0 there)
   s = wave_sum(c * s);
-  const float log_s = M == -INFINITY ? NAN : logf(s), lse = M + log_s;
-  if (tid == 0) write_row<T>(p, row, lse, log_s, t / s);
+  const float log_s = M == -INFINITY ? NAN : logf(s);
+  if (tid == 0) write_row<T>(p, row, M, log_s, t / s);
   if (n == 0) return;
   __syncthreads();
   const uint64_t head = heads[lane];
@@ -363,7 +364,7 @@ __global__ void __launch_bounds__(256) token_logprobs_join_kernel(LogprobParams 
     int r = 0;
 #pragma unroll 8
     for (int j = 0; j < count; ++j) r += cand[j] > key;
-    if (r < n) write_top(p, row, r, key, lse);
+    if (r < n) write_top(p, row, r, key, M, log_s);
   }
 }
 

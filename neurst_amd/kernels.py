@@ -923,7 +923,7 @@ def token_logprobs(logits, tokens, top_n=0):
 
 def token_logprobs_bwd(logits, tokens, lse, entropy, dlogp, dentropy=None, out=None):
     """d(logits) from d(logp) and d(entropy) (either None: zero), with the lse and entropy that token_logprobs returned
-    (nst_token_logprobs_bwd).  out: where to write it; may be logits itself."""
+    (nst_token_logprobs_bwd); probabilities are off by 2^-24 |lse| of themselves.  out: where to write it; may be logits itself."""
     rows, V, ldl = _logit_rows("token_logprobs_bwd", logits, tokens)
     for name, t in (("lse", lse), ("entropy", entropy), ("dlogp", dlogp), ("dentropy", dentropy)):
         if (t is not None or name == "lse") and not _is_vector(t, _F32, rows):

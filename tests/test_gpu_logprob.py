@@ -269,3 +269,25 @@ def test_parts_of_nothing_but_ruled_out_symbols(K, rows, V, mask, dtype):
     tokens = x.argmax(-1)
     assert_forward(K, x, tokens, 6)
     assert_backward(K, x, tokens, torch.randn(rows, generator=g), torch.randn(rows, generator=g))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("offset", [0.0, 1000.0, -1000.0, 20000.0])
+@pytest.mark.parametrize("rows,V", [(7, 1000), (128, 8008), (2, 40000), (4, 128000)])
+def test_log_probabilities_keep_their_bits_under_an_offset(K, rows, V, offset, dtype):
+    """log p = (x - m) - log S: what all logits have in common drops out exactly, so the bound has no |lse| in it.
+        x - m: u |x - m|;    log S: the sum and its terms as in the bound of lse, the logarithm's 4 u log S;    the result: u |log p|
+    (x - m of logits within a factor of two of each other is exact; under a large offset they all are.)"""
+    x = (make_logits(rows, V, torch.float32, "plain", seed=V) + offset).to(dtype)
+    tokens = torch.randint(0, V, (rows,), generator=gen(1))
+    logp, _, _, top_logp, top_ids = (t.cpu() for t in K.token_logprobs(x.to(DEV), tokens.to(DEV), 20))
+    x64 = x.double()
+    d = x64 - x64.amax(-1, keepdim=True)
+    log_s = torch.logsumexp(d, -1)
+    p = (d - log_s[:, None]).exp()
+    H = -(p * (d - log_s[:, None])).sum(-1)
+    t_log_s = U * (V / 256 + 40 + 3 * (H + 8) + 4 * log_s)
+    for ids, got in ((tokens[:, None], logp[:, None]), (top_ids, top_logp)):
+        at = d.gather(1, ids)
+        want = at - log_s[:, None]
+        assert ((got.double() - want).abs() <= t_log_s[:, None] + U * (at.abs() + want.abs())).all()
