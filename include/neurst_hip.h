@@ -603,8 +603,9 @@ typedef struct {
  *   the last one.  cu_new [B + 1]: where the tokens of a request start in that order.  seq_lens [B] = cached + new.
  *   *cursor_out: the first entry of free_pages that is still free.
  * When the free pages run out or a table row is full, the tokens that have no page get slot -1 and are not counted in seq_lens; neither
- * are tokens behind the max_tokens-th, for which there is no slot (max_tokens should be at least sum(new_lens) < 2^31).  The outputs
- * may not be the inputs. */
+ * are tokens behind the max_tokens-th, for which there is no slot (max_tokens should be at least sum(new_lens) < 2^31).  A negative entry of
+ * free_pages is taken like any other and enters the table as -1; its tokens get slot -1 and count in seq_lens, and the attention, which
+ * finds no page, skips them.  The outputs may not be the inputs. */
 int nst_paged_plan(const int32_t* cached_lens, const int32_t* new_lens, int B, int32_t* block_table, int64_t table_stride, int max_pages,
                    const int32_t* free_pages, int n_free, const int32_t* cursor_in, int page_size, int64_t* slots, int64_t max_tokens,
                    int32_t* seq_lens, int32_t* cu_new, int32_t* cursor_out, void* stream);

@@ -147,8 +147,9 @@ __global__ void __launch_bounds__(256) paged_plan_kernel(PlanParams p) {
     }
     const int64_t left = p.n_free - page_base;             // pages behind these do not exist: a senseless length costs no walk
     for (int64_t i = tid; i < n_page && i < left; i += 256) {
-      const int r = find(page_off, (int)i), page = p.free_pages[page_base + i];
-      if (page >= 0) p.table[(int64_t)(b0 + r) * p.table_stride + s_held[r] + (i - page_off[r])] = page;
+      // (an entry that names no page takes the place of whatever the row held here before: that page may be another request's by now)
+      const int r = find(page_off, (int)i);
+      p.table[(int64_t)(b0 + r) * p.table_stride + s_held[r] + (i - page_off[r])] = max(p.free_pages[page_base + i], -1);
     }
   }
   // (64 bits: the last step of a walk over nearly 2^31 tokens passes them; four tokens at a time, so that their pages are looked up together)

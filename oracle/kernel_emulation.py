@@ -611,7 +611,7 @@ def paged_plan(cached_lens, new_lens, block_table, free_pages, cursor, page_size
         held = -(-cached // page_size)
         need = -(-min(cached + new, cap) // page_size) - held
         got = min(max(n_free - at, 0), need)
-        block_table[b, held:held + got] = free_pages[at:at + got]
+        block_table[b, held:held + got] = free_pages[at:at + got].clamp_min(-1)
         at += need
         seq.append(min(cached + min(new, max(int(max_tokens) - t, 0)), (held + got) * page_size))
         for pos in range(cached, cached + new):

@@ -509,3 +509,19 @@ def test_two_calls_at_once(K):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_plan_with_entries_of_the_free_list_that_name_no_page(K):
+    """They enter the table as -1, over whatever a row held there before: their tokens have no slot and attention does not see them."""
+    table = i32([[3, 0, 7], [4, 6, 5], [1, 2, 0]])                                  # (stale entries behind each row's own pages)
+    cached, new, free, cursor = i32([4, 0, 3]), i32([3, 9, 6]), i32([-5, 8, -1, 9, -2 ** 31, 10]), i32([0])
+    want_table = table.clone()
+    want = E.paged_plan(cached, new, want_table, free, cursor, 4, 20)
+    td = table.to(DEV)
+    got = K.paged_plan(cached.to(DEV), new.to(DEV), td, free.to(DEV), cursor.to(DEV), 4, 20)
+    for g, w in zip(got, want):
+        assert torch.equal(g.cpu(), w)
+    assert torch.equal(td.cpu(), want_table) and want_table.tolist() == [[3, -1, 7], [8, -1, 9], [1, -1, 10]]
+    k = torch.randn(11, 4, 1, 64, generator=gen(0))
+    q = torch.randn(3, 2, 64, generator=gen(1))
+    run_attention(K, q, k, k.flip(0).contiguous(), want_table, want[1])

@@ -158,6 +158,14 @@ def test_plan_contract_when_pages_run_out():
     assert table.tolist() == [[9, 5, -1], [6, -1, -1], [-1, -1, -1]]
 
 
+def test_plan_contract_for_free_entries_that_name_no_page():
+    """They count as pages, enter the table as -1 over whatever stood there, and give their tokens no slot."""
+    table = i32([[3, 0, 7], [4, 6, 5]])
+    slots, lens, cu, cursor = E.paged_plan(i32([4, 0]), i32([3, 6]), table, i32([-5, 8, -1]), i32([0]), 4, 10)
+    assert table.tolist() == [[3, -1, 7], [8, -1, 5]]
+    assert slots.tolist() == [-1] * 3 + [32, 33, 34, 35] + [-1] * 3 and lens.tolist() == [7, 6] and cu.tolist() == [0, 3, 9] and cursor.tolist() == [3]
+
+
 def test_attention_contract_for_bad_pages():
     k = torch.randn(2, 2, 1, 8, generator=torch.Generator().manual_seed(0))
     q = torch.ones(3, 1, 8)
