@@ -35,7 +35,7 @@ class PagedKVCache(object):
         self.seq_lens = torch.zeros(rows, dtype=torch.int32, device=device)
         self.cursor = torch.zeros(1, dtype=torch.int32, device=device)
         self.slots = None
-        self.len = 0                                                   # tokens of the longest row, as far as the host was told
+        self.len = 0                                                   # the host's bound of the longest row; exact while all rows grow alike
 
     def reset(self):
         """Every page free again, every row empty."""
@@ -56,16 +56,22 @@ class PagedKVCache(object):
         else:
             setattr(self, name, value)
 
-    def extend(self, new_lens=None, longest=1, max_tokens=None):
+    def extend(self, new_lens=None, longest=1, max_tokens=None, length=None):
         """One new token for every row; or new_lens [rows] int32 on the device, of which none is larger than `longest` and whose sum is at
-        most max_tokens (rows * longest).  The tokens' rows follow each other row after row in append()."""
-        if self.len + longest > self.max_length:
+        most max_tokens (rows * longest).  The tokens' rows follow each other row after row in append().
+        length: what no row is longer than afterwards, where the host knows.  The lengths live on the device, so without it every call is
+        taken to lengthen the longest row by `longest`: rows that grow in turn then seem full before they are (tokens that pass the
+        pages of a row, because `length` was too small, are dropped: nst_paged_plan)."""
+        after = self.len + longest if length is None else length
+        if after < 0:
+            raise ValueError(f"rows of at most {after} tokens")
+        if after > self.max_length:
             raise RuntimeError(f"attention cache of {self.max_length} positions is full")
         self.slots, seq_lens, _, cursor = K.paged_plan(self.seq_lens, self._one_each if new_lens is None else new_lens, self.table, self.free,
                                                        self.cursor, self.page_size, self.rows * longest if max_tokens is None else max_tokens)
         self._keep("seq_lens", seq_lens)
         self._keep("cursor", cursor)
-        self.len += longest
+        self.len = after
 
     def append(self, layer, k, v):
         """k, v [tokens, num_heads, head_dim] of the step's tokens into their slots."""

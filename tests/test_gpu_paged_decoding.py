@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_paged_decoding import _inputs, _toy_model, run_entropy_training
+from test_paged_decoding import _inputs, _toy_model, run_entropy_training, run_rows_that_grow_in_turn
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -57,6 +57,12 @@ def test_graph_replayed_paged_decoding_equals_eager_paged_decoding(fused):
         assert torch.equal(h0, h1) and torch.equal(s0, s1), seed
     dense = BeamSearch(beam_size=3, top_k=2, maximum_decode_length=9, use_graphs=True)
     assert dense(model, inputs)[0].shape == h0.shape and len(model._decode_sessions) == 2      # sessions of their own
+
+
+def test_rows_that_grow_in_turn():
+    """float32, 6 tokens, heads of 8: a score of size 10 is off by (8 + 7) 2^-24 of it, the weights by twice that, the sums by 28 2^-24 -- 2e-5
+    of values of size 4."""
+    run_rows_that_grow_in_turn(DEV, 8e-5)
 
 
 @pytest.mark.parametrize("dtype,tol", [("float32", 1e-5), ("bfloat16", 2.0 ** -6)])

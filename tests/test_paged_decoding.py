@@ -87,6 +87,41 @@ def test_paged_cache_of_rows_with_different_lengths(cpu_kernels):
         PagedKVCache(1, 1, 1, 300, 4, 2, torch.float32, "cpu")
 
 
+def run_rows_that_grow_in_turn(device, tol):
+    """Prompts that arrive one after the other, each for another row: a row is full when IT is, not when the prompts together are as long."""
+    rows, heads, dh, longest = 4, 2, 8, 6
+    cache = PagedKVCache(1, rows, heads, dh, max_length=longest, page_size=4, dtype=torch.float32, device=device)
+    g = torch.Generator().manual_seed(2)
+    hist = [torch.zeros(0, 2, heads, dh) for _ in range(rows)]
+    for new, length in (([5, 0, 0, 0], 5), ([0, 5, 0, 0], 5), ([0, 0, 6, 0], 6), ([1, 0, 0, 3], 6)):
+        kv = torch.randn(sum(new), 2, heads, dh, generator=g)
+        cache.extend(torch.tensor(new, dtype=torch.int32, device=device), longest=max(new), max_tokens=sum(new), length=length)
+        assert cache.len == length
+        cache.append(0, kv[:, 0].to(device), kv[:, 1].to(device))
+        hist = [torch.cat([h, part]) for h, part in zip(hist, kv.split(new))]
+        q = torch.randn(rows, heads, dh, generator=g)
+        out = cache.attend(0, q.to(device)).cpu().double()
+        assert cache.seq_lens.tolist() == [h.shape[0] for h in hist]
+        for r in range(rows):
+            k, v = hist[r][:, 0].double(), hist[r][:, 1].double()
+            want = torch.einsum("ht,thd->hd", torch.softmax(torch.einsum("thd,hd->ht", k, q[r].double()) / dh ** 0.5, -1), v)
+            assert float((out[r] - want).abs().max()) <= tol, (new, r)
+    state = cache.table.clone(), cache.seq_lens.clone(), cache.cursor.clone()
+    with pytest.raises(RuntimeError, match="6 positions is full"):
+        cache.extend(torch.tensor([0, 2, 0, 0], dtype=torch.int32, device=device), longest=2, length=7)
+    with pytest.raises(RuntimeError, match="6 positions is full"):            # the host does not know: the longest row might be the one
+        cache.extend(torch.tensor([0, 1, 0, 0], dtype=torch.int32, device=device))
+    with pytest.raises(ValueError, match="at most -1"):
+        cache.extend(length=-1)
+    assert all(torch.equal(a, b) for a, b in zip(state, (cache.table, cache.seq_lens, cache.cursor))) and cache.len == 6
+    cache.extend(torch.tensor([0, 1, 0, 3], dtype=torch.int32, device=device), longest=3, max_tokens=4, length=6)
+    assert cache.seq_lens.tolist() == [6, 6, 6, 6]
+
+
+def test_rows_that_grow_in_turn(cpu_kernels):
+    run_rows_that_grow_in_turn("cpu", 1e-6)
+
+
 @pytest.mark.parametrize("beam,top_k,alpha,min_len,enable_unk", [(1, 1, 0.6, 0, False), (4, 4, 1.0, 0, False), (3, 2, -1.0, 0, True),
                                                                  (5, 3, 0.0, 6, False), (4, 2, 0.6, 11, False)])
 def test_search_over_the_likeliest_symbols_equals_the_full_search(cpu_kernels, beam, top_k, alpha, min_len, enable_unk):
