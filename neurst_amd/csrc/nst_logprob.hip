@@ -489,7 +489,8 @@ extern "C" int nst_token_logprobs_fwd(const void* logits, const int64_t* tokens,
   else logprobs_launch<float>(p, sp.pieces, (unsigned)(rows * sp.nparts), st);
   if (sp.nparts > 1) {
     NST_CHECK_LAUNCH("nst_token_logprobs_fwd");
-    const size_t held = (size_t)sp.nparts * top_n, lds = sizeof(uint64_t) * (held + (held > MAX_PARTS ? held : MAX_PARTS));      // at most 64 KiB
+    // (64 parts of 64 alternatives: 64 KiB, and the kernel's own word of LDS, of the 160 KiB of a CU)
+    const size_t held = (size_t)sp.nparts * top_n, lds = sizeof(uint64_t) * (held + (held > MAX_PARTS ? held : MAX_PARTS));
     if (dtype == NST_BF16) token_logprobs_join_kernel<bf16_t><<<(unsigned)rows, 256, lds, st>>>(p);
     else token_logprobs_join_kernel<float><<<(unsigned)rows, 256, lds, st>>>(p);
   }

@@ -826,7 +826,8 @@ static int paged_attention_check(const NstPagedAttnDesc* d) {
 //   768 workgroups: what the chip holds at once (three for a CU at 128 .. 168 registers).  24 x 8 float32 heads of up to 2047 tokens: 512 / 768
 //     / 1024 / 2048 workgroups 36.7 / 32.4 / 34.0 / 35.3 us.
 //   Parts of at most 2048 tokens, or the last long requests of a ragged batch run alone (64 requests of 1 .. 8192 tokens, 8 heads: 240 us
-//     without this bound, 223 us with it, 230 us with half of it), and of at least 256.
+//     without this bound, 223 us with it, 230 us with half of it), and of at least 256 in a request as long as the bound (a shorter one of
+//     the batch may come into as many parts, of at least MIN_PART tokens: part_tokens).
 //   Up to 512 tokens a request stays whole (16 x 8 heads: 10.3 us, in parts with the second launch 12.1 us, and a launch less for the host;
 //     up to 256 of float32 with tiles of 16 tokens: 29 x 2 heads of 80, 512 tokens 24.9 us whole, 18.8 in parts),
 //     up to 1024 where there are 128 rows of heads or more (64 x 4: 14.0 against 18.7 us; 8 x 4: 18.3 against 11.6 us, so not for fewer).
