@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(AppendParams p) {
 // With one query head per key / value head 15 of 16 columns of the products are idle: the products take a twentieth of the time a tile
 // needs to arrive, and vector code would have to unpack and multiply every element instead.
 // Bound by memory: 64 requests of 1 .. 8192 tokens, 32 heads of 128 over 8, bf16 (1.07 GB): 220 us and 5 us for the join, 4.9 TB/s (equally
-// long requests 5.4 .. 5.7); 24 requests of up to 2047 tokens, 8 heads of 64, f32 (105 MB): 26 + 4 us; 128 requests of up to 75
+// long requests 5.4 .. 5.7); 24 requests of up to 2047 tokens, 8 heads of 64, f32 (105 MB): 27 + 4 us; 128 requests of up to 75
 // tokens, 4 heads of 64: 5.4 us, the latency of length -> entry -> rows -> join.  More than 16 query heads for a key / value head read it
 // once per 16.
 constexpr int MIN_PART = 128;      // tokens: a tile for each wave; parts are multiples of it
